@@ -1,0 +1,112 @@
+// jinf-b200: operators over a K/V cache for speculative decoding and bounded contexts.
+//
+// No counterpart in the reference, which decodes one token at a time over a cache that only
+// grows (reference src/engine.cpp:690-751). A step that verifies a tree of drafted tokens
+//   1. stores the drafted nodes' K/V rows behind the cached ones (rows n_past + node),
+//   2. runs jinf_b200_tree_attention per layer,
+//   3. once the accepted path is known, credits the cached rows with the attention weight they
+//      received from it (jinf_b200_attention_mass) and moves its rows up behind the cached ones
+//      (jinf_b200_tree_commit),
+//   4. when the cache is full, cuts it back to the rows that matter (jinf_b200_kv_evict).
+//
+// Conventions of jinf/b200.h: device pointers owned by the caller, nothing allocated,
+// asynchronous on `stream`, usable under stream capture, a jinf_status returned. Arguments are
+// checked on the host before any launch. Lengths and lists live on the device, so that a step
+// needs no host round trip; the kernels clamp them to the bounds given here and never read or
+// write outside the views.
+#pragma once
+
+#include <stddef.h>
+#include <stdint.h>
+
+#include "jinf/common.h"
+
+typedef struct CUstream_st* cudaStream_t;
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+// 16-bit types of these operators: JINF_TYPE_F16 (1) and bfloat16 (its GGUF number).
+#define JINF_B200_BF16 30
+
+#define JINF_TREE_MAX_NODES 256
+#define JINF_KV_MAX_SEQS 1024
+
+// K and V rows of n_seqs sequences (or layers, or both): row r of kv head h of sequence s is the
+// head_dim consecutive elements at k + s seq_stride + h head_stride + r row_stride (the same in
+// v). Strides count elements and are multiples of 8; k and v are 16-byte aligned. Any order of
+// the three axes will do ([seq][head][row] as the engine keeps it, [row][head], ...).
+typedef struct jinf_b200_kv {
+    void* k;
+    void* v;
+    int type;        // JINF_TYPE_F16 or JINF_B200_BF16
+    int n_seqs;      // 1..JINF_KV_MAX_SEQS
+    int n_kv_heads;
+    int head_dim;    // 64 or 128
+    int max_ctx;     // rows per sequence and head
+    int64_t seq_stride, head_stride, row_stride;
+} jinf_b200_kv;
+
+// Bit mask of a draft tree (host buffers): parents[t] < t is the node that node t extends, -1 a
+// node that extends the cached text. Writes n_nodes x ceil(n_nodes / 32) words: bit u % 32 of
+// word u / 32 of row t is set when u is t or one of its ancestors.
+jinf_status jinf_b200_tree_mask(const int32_t* parents, int n_nodes, uint32_t* mask);
+
+// Attention of n_nodes new rows of each sequence over its cache. Node t of sequence s attends the
+// rows j < n_past[s] and the tree rows n_past[s] + u for which its mask has bit u, where the
+// caller has stored the nodes' own K/V:
+//   out = sum_j softmax_j(scale q.k_j) v_j,  lse = ln sum_j e^(scale q.k_j)
+// q [n_seqs][n_nodes][n_heads][head_dim] in the cache's type, sequences and nodes q_seq_stride
+// and q_node_stride elements apart (multiples of 8, q 16-byte aligned); query head h reads kv
+// head h / (n_heads / n_kv_heads). out is dense in the same order and type; lse (may be NULL)
+// fp32 [n_seqs][n_nodes][n_heads]. mask: device, [n_nodes][ceil(n_nodes / 32)] words, sequence s's
+// at mask + s mask_seq_stride (0: one mask for all); NULL: node t sees nodes 0..t (n_nodes = 1 is
+// plain decode). A row that attends nothing gives out 0 and lse -inf; what masked and unused
+// cache rows hold, NaN included, does not matter.
+// n_past: device int32 [n_seqs], each clamped to 0..max_past; max_past + n_nodes <= max_ctx.
+// scale > 0. workspace: tree_attention_workspace_bytes for the same arguments, zeroed once before
+// first use, then reusable on the same stream; calls that overlap in time need one each.
+size_t jinf_b200_tree_attention_workspace_bytes(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past);
+jinf_status jinf_b200_tree_attention(void* out, float* lse, const void* q, int64_t q_seq_stride,
+                                     int64_t q_node_stride, int n_heads, int n_nodes, const jinf_b200_kv* kv,
+                                     const int32_t* n_past, int max_past, const uint32_t* mask,
+                                     int64_t mask_seq_stride, float scale, void* workspace, cudaStream_t stream);
+
+// Attention weight each cached row received: for the rows j < n_past[s] + n_nodes,
+//   mass[s][kvh][j] = (j < n_past[s] ? mass[s][kvh][j] : 0)
+//                     + sum_t node_weight[s][t] sum_(h of kvh) e^(scale q_(t,h).k_j - lse[s][t][h])
+// over the (t, j) pairs that tree_attention attends, with its q, mask, scale and lse. mass fp32
+// [n_seqs][n_kv_heads][max_ctx]; node_weight fp32 [n_seqs][n_nodes], NULL for all ones. Nodes of
+// weight 0 (rejected drafts) are left out altogether, and rows with lse = -inf add nothing. Every
+// value has one owner, which adds in a fixed order: equal inputs give equal bits.
+jinf_status jinf_b200_attention_mass(float* mass, const void* q, int64_t q_seq_stride, int64_t q_node_stride,
+                                     int n_heads, int n_nodes, const jinf_b200_kv* kv, const int32_t* n_past,
+                                     int max_past, const float* lse, const uint32_t* mask, int64_t mask_seq_stride,
+                                     const float* node_weight, float scale, cudaStream_t stream);
+
+// Keeps n_keep of the n_rows[s] rows of every (sequence, kv head): the first n_sink, the last
+// n_recent, and of the others those of largest mass (equal ones: the lower row; NaN last). The
+// kept rows keep their order and become rows 0.. of kv_out, their mass that of mass_out
+// [n_seqs][n_kv_heads][kv_out->max_ctx] (may be NULL), their old row numbers ids
+// [n_seqs][n_kv_heads][n_keep], -1 behind the last. n_out[s] = min(n_rows[s], n_keep): a sequence
+// of at most n_keep rows keeps all. n_rows: device, clamped to 0..max_ctx. kv_out NULL (or equal to
+// kv): in place, and mass_out then NULL or equal to mass; otherwise the two caches, and mass and
+// mass_out, do not overlap. 1 <= n_keep <= both max_ctx, n_sink + n_recent <= n_keep. Rows of
+// the output past n_out are left as they are.
+jinf_status jinf_b200_kv_evict(const jinf_b200_kv* kv, const jinf_b200_kv* kv_out, const float* mass, float* mass_out,
+                               const int32_t* n_rows, int32_t* ids, int32_t* n_out, int n_keep, int n_sink,
+                               int n_recent, cudaStream_t stream);
+
+// Moves the accepted path's rows up behind the cached ones, in place: row n_past[s] + accepted[s][i]
+// of K, V and mass (may be NULL) becomes row n_past[s] + i for i < n_accepted[s], and
+// n_out[s] = n_past[s] + n_accepted[s] (n_out may be NULL; it is not n_past itself). accepted:
+// device int32 [n_seqs][accepted_stride], node numbers strictly ascending, as a path's are, at
+// most accepted_stride of them; a number outside 0..n_nodes - 1 moves nothing.
+jinf_status jinf_b200_tree_commit(const jinf_b200_kv* kv, float* mass, const int32_t* n_past, int max_past,
+                                  const int32_t* accepted, int accepted_stride, const int32_t* n_accepted, int n_nodes,
+                                  int32_t* n_out, cudaStream_t stream);
+
+#ifdef __cplusplus
+}
+#endif

@@ -1,0 +1,172 @@
+// Attention weight received by each cached row, sm_100a (jinf_b200_attention_mass):
+//   mass_j = (j < n_past ? mass_j : 0) + sum_r w_r e^(scale q_r.k_j - lse_r)
+// over the query rows r (node, query head of the kv head) that see key j. The rows' softmax is
+// already known by its lse, so one pass over K suffices and every key is independent of the
+// others: a CTA owns 128 keys of a kv head, and each sum has one owner that adds in row order.
+//
+// k_mass_rows: S^T = K Q^T as m16n8k16 fragments, a warp's 16 keys held in registers against the
+// query rows staged through shared memory 32 at a time. Rows of weight 0 are dropped first, so
+// the cost follows the accepted nodes, not the drafted ones.
+#include "kv_ops.cuh"
+
+#include <math.h>
+
+namespace jinf {
+namespace {
+
+constexpr int MW = 8;        // warps of a CTA, 16 keys each
+constexpr int MROWS = 32;    // query rows of a stage
+static_assert(MW * 16 == KV_TILE, "a CTA owns one tile of keys");
+
+template <int HD>
+struct MassSmem {
+    uint8_t q[2][MROWS * HD * 2];
+    float bias[2][MROWS];    // -lse log2 e
+    float weight[2][MROWS];
+    int node[JINF_TREE_MAX_NODES];  // nodes of weight != 0, ascending
+    int n_nodes;
+};
+
+template <bool BF, int HD>
+__global__ void __launch_bounds__(MW * 32)
+    k_mass_rows(const TreeParams p, const float* __restrict__ lse, const float* __restrict__ weight,
+                float* __restrict__ mass) {
+    constexpr int CH = HD / 8, ROWB = HD * 2, KS = HD / 16;
+    __shared__ __align__(128) MassSmem<HD> sm;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int seq = blockIdx.z, head = blockIdx.y;
+    const int past = clamped_past(p, seq), n_keys = past + p.n_nodes;
+    const int tile0 = blockIdx.x * KV_TILE;
+    if (tile0 >= n_keys) return;
+    const uint32_t* mask = p.mask ? p.mask + seq * p.mask_seq : nullptr;
+
+    if (warp == 0) {
+        int n = 0;
+        for (int t0 = 0; t0 < p.n_nodes; t0 += 32) {
+            const int t = t0 + lane;
+            const bool on = t < p.n_nodes && (!weight || weight[(size_t)seq * p.n_nodes + t] != 0.f);
+            const uint32_t b = __ballot_sync(JINF_FULL_MASK, on);
+            if (on) sm.node[n + __popc(b & ((1u << lane) - 1u))] = t;
+            n += __popc(b);
+        }
+        if (lane == 0) sm.n_nodes = n;
+    }
+    __syncthreads();
+    const int rows = sm.n_nodes * p.group, stages = (rows + MROWS - 1) / MROWS;
+
+    auto stage_in = [&](int st) {
+        uint8_t* dst = sm.q[st & 1];
+        for (int i = tid; i < MROWS * CH; i += MW * 32) {
+            const int r = i / CH, c = i % CH, rr = st * MROWS + r;
+            const bool ok = rr < rows;
+            const int t = ok ? sm.node[rr / p.group] : 0, h = head * p.group + (ok ? rr % p.group : 0);
+            cp16_or_zero(smem_u32(dst) + r * ROWB + ((c ^ (r & 7)) << 4),
+                         p.q + (seq * p.q_seq + t * p.q_node + (int64_t)h * HD) * 2 + c * 16, ok);
+        }
+        if (tid < MROWS) {
+            const int rr = st * MROWS + tid;
+            float b = -INFINITY, w = 0.f;
+            if (rr < rows) {
+                const int t = sm.node[rr / p.group], h = head * p.group + rr % p.group;
+                const float x = lse[((size_t)seq * p.n_nodes + t) * p.n_heads + h];
+                if (x != -INFINITY) {  // a row that attended nothing adds nothing
+                    b = -x * LOG2E;
+                    w = weight ? weight[(size_t)seq * p.n_nodes + t] : 1.f;
+                }
+            }
+            sm.bias[st & 1][tid] = b;
+            sm.weight[st & 1][tid] = w;
+        }
+    };
+    if (stages > 0) stage_in(0);
+    cp_commit();
+
+    // this warp's 16 keys as A fragments, straight from memory
+    const int key0 = tile0 + 16 * warp;
+    uint32_t ka[KS][4];
+    {
+        const uint8_t* kb = p.k + (seq * p.kv_seq + head * p.kv_head) * 2;
+        const int ra = key0 + (lane >> 2), rb = ra + 8;
+        const uint32_t* pa = reinterpret_cast<const uint32_t*>(kb + (int64_t)ra * p.kv_row * 2) + (lane & 3);
+        const uint32_t* pb = reinterpret_cast<const uint32_t*>(kb + (int64_t)rb * p.kv_row * 2) + (lane & 3);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            ka[ks][0] = ra < n_keys ? __ldg(pa + 8 * ks) : 0u;
+            ka[ks][1] = rb < n_keys ? __ldg(pb + 8 * ks) : 0u;
+            ka[ks][2] = ra < n_keys ? __ldg(pa + 8 * ks + 4) : 0u;
+            ka[ks][3] = rb < n_keys ? __ldg(pb + 8 * ks + 4) : 0u;
+        }
+    }
+    const float c2 = p.scale * LOG2E;
+    const bool in_tree = key0 + 16 > past;
+    float sum[2] = {0.f, 0.f};
+    for (int st = 0; st < stages; ++st) {
+        if (st + 1 < stages) stage_in(st + 1);
+        cp_commit();
+        cp_wait<1>();
+        __syncthreads();
+        const uint32_t qb = smem_u32(sm.q[st & 1]);
+#pragma unroll
+        for (int n0 = 0; n0 < MROWS; n0 += 16) {
+            float c[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[i][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t b0, b1, b2, b3;
+                const int r = n0 + (lane & 7) + ((lane >> 4) << 3), ch = 2 * ks + ((lane >> 3) & 1);
+                ldsm_x4(qb + r * ROWB + ((ch ^ (r & 7)) << 4), b0, b1, b2, b3);
+                mma16<BF>(c[0], ka[ks], b0, b1);
+                mma16<BF>(c[1], ka[ks], b2, b3);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = n0 + 8 * i + 2 * (lane & 3) + (e & 1);
+                    float x = exp2f(fmaf(c[i][e], c2, sm.bias[st & 1][r]));
+                    if (sm.weight[st & 1][r] == 0.f) x = 0.f;  // behind the last row, or an empty one
+                    if (in_tree) {
+                        const int key = key0 + (lane >> 2) + 8 * (e >> 1), rr = st * MROWS + r;
+                        if (key >= past &&
+                            (key >= n_keys || rr >= rows || !tree_sees(p, mask, sm.node[rr / p.group], key - past)))
+                            x = 0.f;
+                    }
+                    sum[e >> 1] = fmaf(sm.weight[st & 1][r], x, sum[e >> 1]);
+                }
+        }
+        __syncthreads();
+    }
+    cp_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float x = sum[h];
+        x += __shfl_xor_sync(JINF_FULL_MASK, x, 1);
+        x += __shfl_xor_sync(JINF_FULL_MASK, x, 2);
+        const int key = key0 + (lane >> 2) + 8 * h;
+        if ((lane & 3) == 0 && key < n_keys) {
+            float* at = mass + ((size_t)seq * p.n_kv_heads + head) * p.max_ctx + key;
+            *at = key < past ? *at + x : x;
+        }
+    }
+}
+
+template <bool BF, int HD>
+cudaError_t launch_mass(const TreeParams& p, const float* lse, const float* weight, float* mass, cudaStream_t s) {
+    const dim3 grid((unsigned)((p.max_past + p.n_nodes + KV_TILE - 1) / KV_TILE), (unsigned)p.n_kv_heads,
+                    (unsigned)p.n_seqs);
+    k_mass_rows<BF, HD><<<grid, MW * 32, 0, s>>>(p, lse, weight, mass);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, const float* lse, const float* weight,
+                             float* mass, cudaStream_t s) {
+    if (head_dim == 64) return bf ? launch_mass<true, 64>(p, lse, weight, mass, s) : launch_mass<false, 64>(p, lse, weight, mass, s);
+    return bf ? launch_mass<true, 128>(p, lse, weight, mass, s) : launch_mass<false, 128>(p, lse, weight, mass, s);
+}
+
+}  // namespace jinf

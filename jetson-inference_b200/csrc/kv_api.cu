@@ -1,0 +1,171 @@
+// C-ABI of the cache operators (include/jinf/kv_ops.h): argument checks, then the launches.
+#include "kv_ops.cuh"
+#include "jinf/quant.h"
+
+#include <atomic>
+#include <math.h>
+
+using namespace jinf;
+
+namespace jinf {
+int kv_device_sms() {
+    static std::atomic<int> sms[64];  // every writer stores the same value
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int n = sms[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        n = 148;
+        cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        sms[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+}  // namespace jinf
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+static bool kv_ok(const jinf_b200_kv* kv) {
+    return kv && kv->k && kv->v && aligned16(kv->k) && aligned16(kv->v) &&
+           (kv->type == JINF_TYPE_F16 || kv->type == JINF_B200_BF16) && kv->n_seqs >= 1 &&
+           kv->n_seqs <= JINF_KV_MAX_SEQS && kv->n_kv_heads >= 1 && kv->n_kv_heads <= 65535 &&
+           (kv->head_dim == 64 || kv->head_dim == 128) && kv->max_ctx >= 1 && kv->seq_stride % 8 == 0 &&
+           kv->head_stride % 8 == 0 && kv->row_stride % 8 == 0;
+}
+
+static bool tree_shape_ok(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past) {
+    return kv_ok(kv) && n_heads >= 1 && n_heads % kv->n_kv_heads == 0 && n_nodes >= 1 &&
+           n_nodes <= JINF_TREE_MAX_NODES && max_past >= 0 && max_past <= kv->max_ctx - n_nodes &&
+           n_heads / kv->n_kv_heads <= 1024;
+}
+
+static void tree_params(TreeParams* p, const void* q, int64_t q_seq, int64_t q_node, int n_heads, int n_nodes,
+                        const jinf_b200_kv* kv, const int32_t* n_past, int max_past, const uint32_t* mask,
+                        int64_t mask_seq, float scale) {
+    p->k = (const uint8_t*)kv->k;
+    p->v = (const uint8_t*)kv->v;
+    p->q = (const uint8_t*)q;
+    p->kv_seq = kv->seq_stride;
+    p->kv_head = kv->head_stride;
+    p->kv_row = kv->row_stride;
+    p->q_seq = q_seq;
+    p->q_node = q_node;
+    p->n_past = n_past;
+    p->mask = mask;
+    p->mask_seq = mask_seq;
+    p->n_seqs = kv->n_seqs;
+    p->n_heads = n_heads;
+    p->n_kv_heads = kv->n_kv_heads;
+    p->group = n_heads / kv->n_kv_heads;
+    p->n_nodes = n_nodes;
+    p->mask_words = (n_nodes + 31) / 32;
+    p->max_past = max_past;
+    p->max_ctx = kv->max_ctx;
+    p->n_rows = n_nodes * p->group;
+    p->row_blocks = 1;
+    p->block_rows = p->n_rows;
+    p->scale = scale;
+}
+
+static bool query_ok(const void* q, int64_t q_seq, int64_t q_node, float scale) {
+    return q && aligned16(q) && q_seq % 8 == 0 && q_node % 8 == 0 && isfinite(scale) && scale > 0.f;
+}
+
+extern "C" jinf_status jinf_b200_tree_mask(const int32_t* parents, int n_nodes, uint32_t* mask) {
+    if (!parents || !mask || n_nodes < 1 || n_nodes > JINF_TREE_MAX_NODES) return JINF_ERR_INVALID;
+    const int words = (n_nodes + 31) / 32;
+    for (int t = 0; t < n_nodes; ++t)
+        if (parents[t] < -1 || parents[t] >= t) return JINF_ERR_INVALID;
+    for (int t = 0; t < n_nodes; ++t) {
+        for (int w = 0; w < words; ++w) mask[t * words + w] = parents[t] < 0 ? 0u : mask[parents[t] * words + w];
+        mask[t * words + (t >> 5)] |= 1u << (t & 31);
+    }
+    return JINF_OK;
+}
+
+extern "C" size_t jinf_b200_tree_attention_workspace_bytes(const jinf_b200_kv* kv, int n_heads, int n_nodes,
+                                                           int max_past) {
+    if (!tree_shape_ok(kv, n_heads, n_nodes, max_past)) return 0;
+    const TreePlan plan = tree_plan(kv->n_seqs, kv->n_kv_heads, n_nodes * (n_heads / kv->n_kv_heads), n_nodes, max_past,
+                                    kv->head_dim, kv_device_sms());
+    return sizeof(float) * tree_workspace_floats(plan.block_rows, kv->head_dim, plan.n_ctas);
+}
+
+extern "C" jinf_status jinf_b200_tree_attention(void* out, float* lse, const void* q, int64_t q_seq_stride,
+                                                int64_t q_node_stride, int n_heads, int n_nodes,
+                                                const jinf_b200_kv* kv, const int32_t* n_past, int max_past,
+                                                const uint32_t* mask, int64_t mask_seq_stride, float scale,
+                                                void* workspace, cudaStream_t stream) {
+    if (!out || !aligned16(out) || !n_past || !workspace || !aligned16(workspace) || mask_seq_stride < 0 ||
+        !tree_shape_ok(kv, n_heads, n_nodes, max_past) || !query_ok(q, q_seq_stride, q_node_stride, scale))
+        return JINF_ERR_INVALID;
+    TreeParams p;
+    tree_params(&p, q, q_seq_stride, q_node_stride, n_heads, n_nodes, kv, n_past, max_past, mask, mask_seq_stride, scale);
+    const TreePlan plan = tree_plan(p.n_seqs, p.n_kv_heads, p.n_rows, n_nodes, max_past, kv->head_dim, kv_device_sms());
+    p.row_blocks = plan.row_blocks;
+    p.block_rows = plan.block_rows;
+    return tree_attn_launch(p, plan, kv->type == JINF_B200_BF16, kv->head_dim, out, lse, (float*)workspace, stream) ==
+                   cudaSuccess
+               ? JINF_OK
+               : JINF_ERR_CUDA;
+}
+
+extern "C" jinf_status jinf_b200_attention_mass(float* mass, const void* q, int64_t q_seq_stride,
+                                                int64_t q_node_stride, int n_heads, int n_nodes,
+                                                const jinf_b200_kv* kv, const int32_t* n_past, int max_past,
+                                                const float* lse, const uint32_t* mask, int64_t mask_seq_stride,
+                                                const float* node_weight, float scale, cudaStream_t stream) {
+    if (!mass || !n_past || !lse || mask_seq_stride < 0 || !tree_shape_ok(kv, n_heads, n_nodes, max_past) ||
+        !query_ok(q, q_seq_stride, q_node_stride, scale))
+        return JINF_ERR_INVALID;
+    TreeParams p;
+    tree_params(&p, q, q_seq_stride, q_node_stride, n_heads, n_nodes, kv, n_past, max_past, mask, mask_seq_stride, scale);
+    return attn_mass_launch(p, kv->type == JINF_B200_BF16, kv->head_dim, lse, node_weight, mass, stream) == cudaSuccess
+               ? JINF_OK
+               : JINF_ERR_CUDA;
+}
+
+static KvPlanes planes(const jinf_b200_kv* kv) {
+    KvPlanes p;
+    p.k = (uint8_t*)kv->k;
+    p.v = (uint8_t*)kv->v;
+    p.seq = kv->seq_stride * 2;
+    p.head = kv->head_stride * 2;
+    p.row = kv->row_stride * 2;
+    p.max_ctx = kv->max_ctx;
+    return p;
+}
+
+extern "C" jinf_status jinf_b200_kv_evict(const jinf_b200_kv* kv, const jinf_b200_kv* kv_out, const float* mass,
+                                          float* mass_out, const int32_t* n_rows, int32_t* ids, int32_t* n_out,
+                                          int n_keep, int n_sink, int n_recent, cudaStream_t stream) {
+    if (!kv_out) kv_out = kv;
+    if (!kv_ok(kv) || !kv_ok(kv_out) || !mass || !n_rows || !ids || n_keep < 1 || n_keep > kv->max_ctx ||
+        n_keep > kv_out->max_ctx || n_sink < 0 || n_recent < 0 || n_sink > n_keep || n_recent > n_keep - n_sink ||
+        n_out == n_rows)
+        return JINF_ERR_INVALID;
+    if (kv_out->type != kv->type || kv_out->n_seqs != kv->n_seqs || kv_out->n_kv_heads != kv->n_kv_heads ||
+        kv_out->head_dim != kv->head_dim)
+        return JINF_ERR_INVALID;
+    const bool in_place = kv_out->k == kv->k || kv_out->v == kv->v;
+    if (in_place && (kv_out->k != kv->k || kv_out->v != kv->v || kv_out->seq_stride != kv->seq_stride ||
+                     kv_out->head_stride != kv->head_stride || kv_out->row_stride != kv->row_stride ||
+                     kv_out->max_ctx != kv->max_ctx))
+        return JINF_ERR_INVALID;
+    if (mass_out && (mass_out == mass) != in_place) return JINF_ERR_INVALID;
+    return kv_evict_launch(planes(kv), planes(kv_out), in_place, mass, mass_out, n_rows, ids, n_out, kv->n_seqs,
+                           kv->n_kv_heads, kv->head_dim * 2, n_keep, n_sink, n_recent, stream) == cudaSuccess
+               ? JINF_OK
+               : JINF_ERR_CUDA;
+}
+
+extern "C" jinf_status jinf_b200_tree_commit(const jinf_b200_kv* kv, float* mass, const int32_t* n_past, int max_past,
+                                             const int32_t* accepted, int accepted_stride, const int32_t* n_accepted,
+                                             int n_nodes, int32_t* n_out, cudaStream_t stream) {
+    if (!kv_ok(kv) || !n_past || !accepted || !n_accepted || n_nodes < 1 || n_nodes > JINF_TREE_MAX_NODES ||
+        max_past < 0 || max_past > kv->max_ctx - n_nodes || accepted_stride < 1 || n_out == n_past)
+        return JINF_ERR_INVALID;
+    return tree_commit_launch(planes(kv), mass, n_past, max_past, accepted, accepted_stride, n_accepted, n_nodes, n_out,
+                              kv->n_seqs, kv->n_kv_heads, kv->head_dim * 2, stream) == cudaSuccess
+               ? JINF_OK
+               : JINF_ERR_CUDA;
+}

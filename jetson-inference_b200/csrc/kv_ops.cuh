@@ -1,0 +1,186 @@
+// Shared pieces of the cache operators (tree_attn.cu, attn_mass.cu, kv_evict.cu): the device view
+// of a K/V cache, 16-bit fragments and masks, and the division of a launch's work.
+#pragma once
+
+#include "common.cuh"
+#include "mma_f16.cuh"
+#include "jinf/kv_ops.h"
+
+#include <cuda_bf16.h>
+
+namespace jinf {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+
+// One launch's cache and queries (fields as in jinf/kv_ops.h; strides in elements).
+struct TreeParams {
+    const uint8_t* k;
+    const uint8_t* v;
+    const uint8_t* q;
+    int64_t kv_seq, kv_head, kv_row;
+    int64_t q_seq, q_node;
+    const int32_t* n_past;
+    const uint32_t* mask;
+    int64_t mask_seq;
+    int n_seqs, n_heads, n_kv_heads, group, n_nodes, mask_words, max_past, max_ctx;
+    int n_rows;      // query rows of a kv head: n_nodes * group, row r = node r / group, head r % group
+    int row_blocks;  // blocks of query rows a kv head's rows are divided into
+    int block_rows;  // rows of a block (the last may have fewer)
+    float scale;
+};
+
+__device__ __forceinline__ int clamped_past(const TreeParams& p, int seq) {
+    return min(max(p.n_past[seq], 0), p.max_past);
+}
+
+// Whether node t sees tree row u (both < n_nodes); `mask`: the sequence's words or null.
+__device__ __forceinline__ bool tree_sees(const TreeParams& p, const uint32_t* mask, int t, int u) {
+    return mask ? (mask[t * p.mask_words + (u >> 5)] >> (u & 31)) & 1u : u <= t;
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        return pack_h2(a, b);
+    }
+}
+template <bool BF>
+__device__ __forceinline__ float to_f32(uint16_t x) {
+    if constexpr (BF) return __uint_as_float((uint32_t)x << 16);
+    else return __half2float(__ushort_as_half(x));
+}
+// One of the two 16-bit values of a word is an infinity or a NaN (all exponent bits set).
+template <bool BF>
+__device__ __forceinline__ bool nonfinite2(uint32_t w) {
+    constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u;
+    return (w & E) == E || ((w >> 16) & E) == E;
+}
+
+// c += A B, m16n8k16, fp32 accumulators
+template <bool BF>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        mma_f16(c, a[0], a[1], a[2], a[3], b0, b1);
+}
+
+// 16 bytes global -> shared, zeros instead when !valid (src is not read then)
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ---- division of the work ----
+//
+// A unit is one (sequence, kv head, row block); it has ceil((n_past + n_nodes) / KV_TILE) key
+// tiles. The tiles of all units, in order, are dealt to the CTAs in equal contiguous shares, so
+// the division is even whatever the sequences' lengths, and is computed on the device from them.
+constexpr int KV_TILE = 128;
+
+__device__ __forceinline__ int seq_tiles(const TreeParams& p, int seq) {
+    return (clamped_past(p, seq) + p.n_nodes + KV_TILE - 1) / KV_TILE;
+}
+
+// prefix[s] = tiles of one (kv head, row block) over the sequences before s, s <= n_seqs; all
+// threads of the CTA call it. `prefix` holds n_seqs + 1 ints of shared memory.
+__device__ __forceinline__ void tile_prefix(const TreeParams& p, int* prefix) {
+    if (threadIdx.x < 32) {
+        int base = 0;
+        for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+            const int s = s0 + (int)threadIdx.x;
+            int t = s < p.n_seqs ? seq_tiles(p, s) : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(JINF_FULL_MASK, t, o);
+                if ((int)threadIdx.x >= o) t += x;
+            }
+            if (s < p.n_seqs) prefix[s + 1] = base + t;
+            base += __shfl_sync(JINF_FULL_MASK, t, 31);
+        }
+        if (threadIdx.x == 0) prefix[0] = 0;
+    }
+    __syncthreads();
+}
+
+struct Unit {
+    int seq, head, block;
+    int64_t first;  // the unit's first tile, in the numbering over all units
+    int tiles;
+};
+
+// The unit that holds global tile `t` (units ordered by sequence, head, block).
+__device__ __forceinline__ Unit unit_of(const TreeParams& p, const int* prefix, int64_t t) {
+    const int per = p.n_kv_heads * p.row_blocks;
+    int lo = 0, hi = p.n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((int64_t)prefix[mid] * per <= t) lo = mid; else hi = mid - 1;
+    }
+    Unit u;
+    u.seq = lo;
+    u.tiles = prefix[lo + 1] - prefix[lo];
+    const int64_t in_seq = t - (int64_t)prefix[lo] * per;
+    const int hb = (int)(in_seq / u.tiles);
+    u.head = hb / p.row_blocks;
+    u.block = hb % p.row_blocks;
+    u.first = t - in_seq + (int64_t)hb * u.tiles;
+    return u;
+}
+
+// CTAs that get a share: none is empty, so the parts of a unit are those of consecutive CTAs.
+__device__ __forceinline__ int share_count(int64_t total, int n_ctas) { return (int)min((int64_t)n_ctas, total); }
+__device__ __forceinline__ int64_t share_start(int64_t total, int cta, int n_ctas) { return total * cta / n_ctas; }
+// The CTA whose share holds tile t.
+__device__ __forceinline__ int share_owner(int64_t total, int64_t t, int n_ctas) {
+    int c = (int)((t * n_ctas) / total);
+    while (c + 1 < n_ctas && share_start(total, c + 1, n_ctas) <= t) ++c;
+    while (c > 0 && share_start(total, c, n_ctas) > t) --c;
+    return c;
+}
+
+int kv_device_sms();  // SMs of the current device (cached per device)
+
+// ---- launches (return a cudaError_t; arguments already checked) ----
+
+// fp32 scratch of a tree attention: partial rows of the units that several CTAs share. CTA c's
+// two slots (a unit begun by an earlier CTA; one it hands on) hold block_rows rows each.
+size_t tree_workspace_floats(int block_rows, int head_dim, int n_ctas);
+struct TreePlan {
+    int row_blocks, block_rows, n_ctas;
+    bool splits;  // some unit may be shared by several CTAs
+};
+TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int head_dim, int sms);
+cudaError_t tree_attn_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, void* out, float* lse,
+                             float* ws, cudaStream_t s);
+
+cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, const float* lse, const float* weight,
+                             float* mass, cudaStream_t s);
+
+struct KvPlanes {  // K and V with their strides in bytes
+    uint8_t* k;
+    uint8_t* v;
+    int64_t seq, head, row;
+    int max_ctx;
+};
+cudaError_t kv_evict_launch(const KvPlanes& src, const KvPlanes& dst, bool in_place, const float* mass, float* mass_out,
+                            const int32_t* n_rows, int32_t* ids, int32_t* n_out, int n_seqs, int n_kv_heads,
+                            int row_bytes, int n_keep, int n_sink, int n_recent, cudaStream_t s);
+cudaError_t tree_commit_launch(const KvPlanes& kv, float* mass, const int32_t* n_past, int max_past,
+                               const int32_t* accepted, int accepted_stride, const int32_t* n_accepted, int n_nodes,
+                               int32_t* n_out, int n_seqs, int n_kv_heads, int row_bytes, cudaStream_t s);
+
+}  // namespace jinf

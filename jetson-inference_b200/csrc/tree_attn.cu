@@ -1,0 +1,469 @@
+// Attention of a tree of drafted tokens over a K/V cache, sm_100a (jinf_b200_tree_attention).
+//
+//   s_rj = scale q_r.k_j,  m_r = max_j s_rj,  l_r = sum_j e^(s_rj - m_r),
+//   out_r = sum_j e^(s_rj - m_r) v_j / l_r,   lse_r = m_r + ln l_r
+// over the rows j that query row r (node r / group, query head r % group of the kv head) sees:
+// all cached ones and its ancestors among the tree's own rows. One pass over K and V with the
+// running (m, l); the rows of all nodes and of all query heads of a kv head share that pass.
+//
+// k_tree_rows: up to 32 rows of a kv head at a time. A warp streams its own 16-key chunks (K and
+// V, 16-byte asynchronous copies, a private ring, no CTA barrier), s = Q K^T and O += P V as
+// m16n8k16 fragments with the probabilities staying in registers. Units are dealt to the CTAs
+// by tile (kv_ops.cuh); a CTA's eight warps join their (m, l, O) in shared memory, and
+// k_tree_merge joins what several CTAs hold of one unit.
+#include "kv_ops.cuh"
+
+#include <math.h>
+
+#include <type_traits>
+
+namespace jinf {
+namespace {
+
+constexpr int TW = 8;        // warps of a CTA
+constexpr int TS = 3;        // ring stages of a warp
+constexpr int WKEYS = 16;    // keys of a warp's chunk: KV_TILE / TW
+static_assert(TW * WKEYS == KV_TILE, "a tile is one chunk of each warp");
+
+template <int HD, int MT>
+struct RowsSmem {
+    static constexpr int RING = TW * TS * 2 * WKEYS * HD * 2;     // bytes
+    static constexpr int JOIN = TW * 16 * MT * (HD + 2) * 4;      // the warps' (O, m, l) at the end of a unit
+    static constexpr int Q = 16 * MT * HD * 2;
+    static constexpr int UNION = RING > JOIN ? RING : JOIN;
+    static constexpr int TOTAL = UNION + Q;                       // + prefix
+};
+
+// The partial rows of CTA c's slot: [block_rows][HD] O (unnormalised, of scale e^-m), then
+// [block_rows] m (of the unscaled scores) and [block_rows] l; slots start on 16 bytes.
+__host__ __device__ __forceinline__ size_t slot_floats(int block_rows, int hd) {
+    return ((size_t)block_rows * (hd + 2) + 3) & ~(size_t)3;
+}
+
+template <bool BF, int HD, int MT>
+__global__ void __launch_bounds__(TW * 32, 1)
+    k_tree_rows(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, float* __restrict__ ws) {
+    using SM = RowsSmem<HD, MT>;
+    constexpr int CH = HD / 8;       // 16-byte chunks of a row
+    constexpr int ROWB = HD * 2;     // bytes of a row
+    constexpr int KS = HD / 16;      // k steps of q.k
+    constexpr int NT = HD / 8;       // column tiles of O
+    extern __shared__ __align__(128) uint8_t sm[];
+    float* join = reinterpret_cast<float*>(sm);
+    uint8_t* sq = sm + SM::UNION;
+    int* prefix = reinterpret_cast<int*>(sm + SM::TOTAL);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t ring = smem_u32(sm) + warp * (TS * 2 * WKEYS * ROWB);
+
+    tile_prefix(p, prefix);
+    const int64_t total = (int64_t)prefix[p.n_seqs] * p.n_kv_heads * p.row_blocks;
+    const int n_ctas = share_count(total, gridDim.x);
+    if ((int)blockIdx.x >= n_ctas) return;
+    const int64_t begin = share_start(total, blockIdx.x, n_ctas), end = share_start(total, blockIdx.x + 1, n_ctas);
+    const float c2 = p.scale * LOG2E;
+
+    for (int64_t at = begin; at < end;) {
+        const Unit u = unit_of(p, prefix, at);
+        const int t0 = (int)(at - u.first);
+        const int t1 = (int)min((int64_t)u.tiles, end - u.first);
+        at = u.first + t1;
+        const int past = clamped_past(p, u.seq), n_keys = past + p.n_nodes;
+        const int row0 = u.block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
+        const uint32_t* mask = p.mask ? p.mask + u.seq * p.mask_seq : nullptr;
+        const int64_t kvo = (u.seq * p.kv_seq + u.head * p.kv_head) * 2;
+
+        // the block's query rows, zeros behind the last (16-byte chunk c of row r at c ^ (r & 7))
+        for (int i = tid; i < 16 * MT * CH; i += TW * 32) {
+            const int r = i / CH, c = i % CH, rr = row0 + r;
+            const bool ok = r < rows;
+            const int node = ok ? rr / p.group : 0, g = ok ? rr % p.group : 0;
+            cp16_or_zero(smem_u32(sq) + r * ROWB + ((c ^ (r & 7)) << 4),
+                         p.q + (u.seq * p.q_seq + node * p.q_node + (int64_t)(u.head * p.group + g) * HD) * 2 + c * 16, ok);
+        }
+        cp_commit();
+
+        auto copy_chunk = [&](int t) {  // this warp's keys of tile t into its ring slot
+            const uint32_t kd = ring + (uint32_t)((t - t0) % TS) * (2 * WKEYS * ROWB), vd = kd + WKEYS * ROWB;
+            const int key0 = t * KV_TILE + warp * WKEYS;
+#pragma unroll
+            for (int i = lane; i < WKEYS * CH; i += 32) {
+                const int r = i / CH, c = i % CH;
+                const bool ok = key0 + r < n_keys;
+                const int64_t off = kvo + (ok ? (int64_t)(key0 + r) * p.kv_row * 2 : 0) + c * 16;
+                const uint32_t d = r * ROWB + ((c ^ (r & 7)) << 4);
+                cp16_or_zero(kd + d, p.k + off, ok);
+                cp16_or_zero(vd + d, p.v + off, ok);
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < TS - 1; ++s) {
+            if (t0 + s < t1) copy_chunk(t0 + s);
+            cp_commit();
+        }
+        cp_wait<TS - 1>();  // the query rows
+        __syncthreads();
+
+        float o[MT][NT][4], m[MT][2], l[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { m[mt][h] = -INFINITY; l[mt][h] = 0.f; }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+        }
+
+        for (int t = t0; t < t1; ++t) {
+            if (t + TS - 1 < t1) copy_chunk(t + TS - 1);
+            cp_commit();
+            cp_wait<TS - 1>();
+            __syncwarp();
+            const uint32_t kd = ring + (uint32_t)((t - t0) % TS) * (2 * WKEYS * ROWB), vd = kd + WKEYS * ROWB;
+            const int key0 = t * KV_TILE + warp * WKEYS;
+            if (key0 >= n_keys) continue;  // the warp's keys of a unit's last tile may all be past the end
+            float s[MT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                uint32_t b0, b1, b2, b3;  // keys 0-7 and 8-15 of the chunk
+                {
+                    const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * ks + ((lane >> 3) & 1);
+                    ldsm_x4(kd + r * ROWB + ((c ^ (r & 7)) << 4), b0, b1, b2, b3);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    uint32_t a[4];
+                    const int r = 16 * mt + (lane & 15), c = 2 * ks + (lane >> 4);
+                    ldsm_x4(smem_u32(sq) + r * ROWB + ((c ^ (r & 7)) << 4), a[0], a[1], a[2], a[3]);
+                    mma16<BF>(s[mt][0], a, b0, b1);
+                    mma16<BF>(s[mt][1], a, b2, b3);
+                }
+            }
+            // Keys among the tree's own rows: -inf where the row does not see them. A masked key's V
+            // would still enter O as 0 * v, so values of these keys that are not finite are taken
+            // out of the chunk and added, as themselves, to the rows that do see their key.
+            uint32_t bad = 0;  // keys of the chunk with such values
+            if (key0 + WKEYS > past) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int key = key0 + 8 * n + 2 * (lane & 3) + (e & 1);
+                            const int r = 16 * mt + (lane >> 2) + 8 * (e >> 1);
+                            const bool see = r < rows && key < n_keys &&
+                                             (key < past || tree_sees(p, mask, (row0 + r) / p.group, key - past));
+                            if (!see) s[mt][n][e] = -INFINITY;
+                        }
+                for (int i = lane; i < WKEYS * CH; i += 32) {
+                    const int r = i / CH;
+                    if (key0 + r < past) continue;
+                    const uint32_t a = vd + i * 16;
+                    uint32_t w[4];
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+                    if (nonfinite2<BF>(w[0]) || nonfinite2<BF>(w[1]) || nonfinite2<BF>(w[2]) || nonfinite2<BF>(w[3])) {
+                        bad |= 1u << r;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            if (nonfinite2<BF>(w[x] & 0xFFFFu)) w[x] &= 0xFFFF0000u;
+                            if (nonfinite2<BF>(w[x] & 0xFFFF0000u)) w[x] &= 0xFFFFu;
+                        }
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                                     "r"(w[3]) : "memory");
+                    }
+                }
+                bad = __reduce_or_sync(JINF_FULL_MASK, bad);
+                __syncwarp();
+            }
+            uint32_t pa[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float mx = fmaxf(fmaxf(s[mt][0][2 * h], s[mt][0][2 * h + 1]), fmaxf(s[mt][1][2 * h], s[mt][1][2 * h + 1]));
+                    mx = fmaxf(mx, __shfl_xor_sync(JINF_FULL_MASK, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(JINF_FULL_MASK, mx, 2));
+                    const float mn = fmaxf(m[mt][h], mx);
+                    const float base = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every e is e^-inf = 0
+                    const float corr = exp2f((m[mt][h] - base) * c2);
+                    m[mt][h] = mn;
+                    float sum = 0.f;
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float x = exp2f((s[mt][n][2 * h + e] - base) * c2);
+                            s[mt][n][2 * h + e] = x;
+                            sum += x;
+                        }
+                    l[mt][h] = l[mt][h] * corr + sum;
+                    if (__any_sync(JINF_FULL_MASK, corr != 1.f)) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            o[mt][n][2 * h] *= corr;
+                            o[mt][n][2 * h + 1] *= corr;
+                        }
+                    }
+                }
+                // P as the A operand: the accumulator layout of two 8-key tiles is that of one 16-key A
+                // tile. Rounding p <= 1 to the cache's type costs about what rounding out to it does.
+                pa[mt][0] = pack2<BF>(s[mt][0][0], s[mt][0][1]);
+                pa[mt][1] = pack2<BF>(s[mt][0][2], s[mt][0][3]);
+                pa[mt][2] = pack2<BF>(s[mt][1][0], s[mt][1][1]);
+                pa[mt][3] = pack2<BF>(s[mt][1][2], s[mt][1][3]);
+            }
+            while (bad) {
+                const int r = __ffs(bad) - 1, key = key0 + r;
+                bad &= bad - 1;
+                const uint16_t* vr = reinterpret_cast<const uint16_t*>(p.v + kvo + (int64_t)key * p.kv_row * 2);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = to_f32<BF>(vr[8 * n + 2 * (lane & 3) + (e & 1)]);
+                        if (fabsf(x) <= 3.4028235e38f) continue;  // finite (false for NaN)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            const int row = 16 * mt + (lane >> 2) + 8 * (e >> 1);
+                            if (row < rows && tree_sees(p, mask, (row0 + row) / p.group, key - past))
+                                o[mt][n][e] += x;
+                        }
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t b0, b1, b2, b3;
+                const int r = lane & 15, c = n + (lane >> 4);
+                ldsm_x4_t(vd + r * ROWB + ((c ^ (r & 7)) << 4), b0, b1, b2, b3);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma16<BF>(o[mt][n], pa[mt], b0, b1);
+                    mma16<BF>(o[mt][n + 1], pa[mt], b2, b3);
+                }
+            }
+            __syncwarp();  // the chunk is read: the next copies may take its slot
+        }
+        cp_wait<0>();
+        __syncthreads();  // every warp is done with its ring and with the queries
+
+        // join the warps
+        float* jm = join + TW * 16 * MT * HD;
+        float* jl = jm + TW * 16 * MT;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float sum = l[mt][h];
+                sum += __shfl_xor_sync(JINF_FULL_MASK, sum, 1);
+                sum += __shfl_xor_sync(JINF_FULL_MASK, sum, 2);
+                const int r = 16 * mt + (lane >> 2) + 8 * h;
+                if ((lane & 3) == 0) {
+                    jm[warp * 16 * MT + r] = m[mt][h];
+                    jl[warp * 16 * MT + r] = sum;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    *reinterpret_cast<float2*>(join + ((size_t)warp * 16 * MT + r) * HD + 8 * n + 2 * (lane & 3)) =
+                        make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
+            }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == u.tiles;
+        float* part = ws + ((size_t)blockIdx.x * 2 + (t0 == 0 ? 1 : 0)) * slot_floats(p.block_rows, HD);
+        for (int i = tid; i < rows * (HD / 4); i += TW * 32) {
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < TW; ++w) M = fmaxf(M, jm[w * 16 * MT + r]);
+            const float base = M == -INFINITY ? 0.f : M;
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            float L = 0.f;
+#pragma unroll
+            for (int w = 0; w < TW; ++w) {
+                const float f = exp2f((jm[w * 16 * MT + r] - base) * c2);
+                const float4 x = *reinterpret_cast<const float4*>(join + ((size_t)w * 16 * MT + r) * HD + d);
+                L = fmaf(jl[w * 16 * MT + r], f, L);
+                a.x = fmaf(x.x, f, a.x);
+                a.y = fmaf(x.y, f, a.y);
+                a.z = fmaf(x.z, f, a.z);
+                a.w = fmaf(x.w, f, a.w);
+            }
+            if (whole) {
+                const int rr = row0 + r;
+                const size_t orow = ((size_t)u.seq * p.n_nodes + rr / p.group) * p.n_heads + u.head * p.group + rr % p.group;
+                const float inv = L > 0.f ? 1.f / L : L == 0.f ? 1.f : L;  // an empty row stays 0, NaN stays NaN
+                const uint2 w2 = make_uint2(pack2<BF>(a.x * inv, a.y * inv), pack2<BF>(a.z * inv, a.w * inv));
+                *reinterpret_cast<uint2*>(out + orow * HD + d) = w2;
+                if (lse && d == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
+            } else {
+                *reinterpret_cast<float4*>(part + (size_t)r * HD + d) = a;
+                if (d == 0) {
+                    part[(size_t)p.block_rows * HD + r] = M;
+                    part[(size_t)p.block_rows * (HD + 1) + r] = L;
+                }
+            }
+        }
+        __syncthreads();  // the join area is the ring of the next unit
+    }
+    pdl_trigger();
+}
+
+constexpr int MERGE_WARPS = 8;
+
+// Joins the parts of the units that several CTAs share: one warp per row, each part's O scaled by
+// e^(m_part - m) and added in the order of the CTAs.
+template <bool BF, int HD>
+__global__ void __launch_bounds__(MERGE_WARPS * 32)
+    k_tree_merge(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, const float* __restrict__ ws,
+                 int n_ctas) {
+    extern __shared__ int prefix[];
+    constexpr int V = HD / 32;  // values of a lane
+    tile_prefix(p, prefix);
+    const int64_t total = (int64_t)prefix[p.n_seqs] * p.n_kv_heads * p.row_blocks;
+    n_ctas = share_count(total, n_ctas);
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);  // over (seq, kv head, row)
+    const bool ok = row < (int64_t)p.n_seqs * p.n_kv_heads * p.n_rows;
+    int c0 = 0, c1 = 0, r = 0, rr = 0, seq = 0, head = 0;
+    int64_t first = 0;
+    if (ok) {
+        rr = (int)(row % p.n_rows);
+        const int64_t sh = row / p.n_rows;
+        head = (int)(sh % p.n_kv_heads);
+        seq = (int)(sh / p.n_kv_heads);
+        const int tiles = prefix[seq + 1] - prefix[seq], block = rr / p.block_rows;
+        r = rr % p.block_rows;
+        first = ((int64_t)prefix[seq] * p.n_kv_heads + (int64_t)head * tiles) * p.row_blocks + (int64_t)block * tiles;
+        c0 = share_owner(total, first, n_ctas);
+        c1 = share_owner(total, first + tiles - 1, n_ctas);
+    }
+    pdl_wait();  // the parts below are the previous kernel's
+    if (c0 == c1) return;
+    const size_t sf = slot_floats(p.block_rows, HD);
+    const float c2 = p.scale * LOG2E;
+    float M = -INFINITY, L = 0.f, a[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[v] = 0.f;
+    constexpr int B = 8;
+    for (int cb = c0; cb <= c1; cb += B) {
+        float pm[B], pl[B], po[B][V];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int c = cb + i;
+            pm[i] = -INFINITY;
+            pl[i] = 0.f;
+            if (c <= c1) {
+                // the CTA that begins the unit kept it in its second slot, the others in their first
+                const float* part = ws + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * sf;
+                pm[i] = __ldcg(part + (size_t)p.block_rows * HD + r);
+                pl[i] = __ldcg(part + (size_t)p.block_rows * (HD + 1) + r);
+                if constexpr (V == 4) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4*>(part + (size_t)r * HD) + lane);
+                    po[i][0] = x.x; po[i][1] = x.y; po[i][2] = x.z; po[i][3] = x.w;
+                } else {
+                    const float2 x = __ldcg(reinterpret_cast<const float2*>(part + (size_t)r * HD) + lane);
+                    po[i][0] = x.x; po[i][1] = x.y;
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) po[i][v] = 0.f;
+            }
+        }
+        float mn = M;
+#pragma unroll
+        for (int i = 0; i < B; ++i) mn = fmaxf(mn, pm[i]);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float corr = exp2f((M - base) * c2);
+        M = mn;
+        L *= corr;
+#pragma unroll
+        for (int v = 0; v < V; ++v) a[v] *= corr;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const float f = exp2f((pm[i] - base) * c2);
+            L = fmaf(pl[i], f, L);
+#pragma unroll
+            for (int v = 0; v < V; ++v) a[v] = fmaf(po[i][v], f, a[v]);
+        }
+    }
+    const size_t orow = ((size_t)seq * p.n_nodes + rr / p.group) * p.n_heads + head * p.group + rr % p.group;
+    const float inv = L > 0.f ? 1.f / L : L == 0.f ? 1.f : L;
+    if constexpr (V == 4)
+        *reinterpret_cast<uint2*>(out + orow * HD + lane * 4) =
+            make_uint2(pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv));
+    else
+        *reinterpret_cast<uint32_t*>(out + orow * HD + lane * 2) = pack2<BF>(a[0] * inv, a[1] * inv);
+    if (lse && lane == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
+}
+
+template <typename K>
+cudaError_t launch(K kernel, dim3 grid, int threads, size_t smem, bool pdl, cudaStream_t s, const TreeParams& p,
+                   uint16_t* out, float* lse, float* ws, int n_ctas) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl ? 1 : 0;
+    if constexpr (std::is_invocable_v<K, const TreeParams, uint16_t*, float*, const float*, int>)
+        return cudaLaunchKernelEx(&cfg, kernel, p, out, lse, (const float*)ws, n_ctas);
+    else
+        return cudaLaunchKernelEx(&cfg, kernel, p, out, lse, ws);
+}
+
+template <bool BF, int HD, int MT>
+cudaError_t launch_rows(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* ws, cudaStream_t s) {
+    const size_t smem = RowsSmem<HD, MT>::TOTAL + (size_t)(JINF_KV_MAX_SEQS + 1) * sizeof(int);
+    cudaError_t e = cudaFuncSetAttribute(k_tree_rows<BF, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch(k_tree_rows<BF, HD, MT>, dim3(plan.n_ctas), TW * 32, smem, false, s, p, out, lse, ws, plan.n_ctas);
+}
+
+template <bool BF, int HD>
+cudaError_t launch_all(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* ws, cudaStream_t s) {
+    cudaError_t e = plan.block_rows <= 16 ? launch_rows<BF, HD, 1>(p, plan, out, lse, ws, s)
+                                          : launch_rows<BF, HD, 2>(p, plan, out, lse, ws, s);
+    if (e != cudaSuccess || !plan.splits) return e;
+    const int64_t rows = (int64_t)p.n_seqs * p.n_kv_heads * p.n_rows;
+    return launch(k_tree_merge<BF, HD>, dim3((unsigned)((rows + MERGE_WARPS - 1) / MERGE_WARPS)), MERGE_WARPS * 32,
+                  (size_t)(p.n_seqs + 1) * sizeof(int), true, s, p, out, lse, ws, plan.n_ctas);
+}
+
+}  // namespace
+
+size_t tree_workspace_floats(int block_rows, int head_dim, int n_ctas) {
+    return (size_t)n_ctas * 2 * slot_floats(block_rows, head_dim);
+}
+
+TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int head_dim, int sms) {
+    (void)head_dim;
+    TreePlan t;
+    t.row_blocks = (n_rows + 31) / 32;
+    t.block_rows = (n_rows + t.row_blocks - 1) / t.row_blocks;
+    t.row_blocks = (n_rows + t.block_rows - 1) / t.block_rows;
+    const int64_t tiles = (max_past + n_nodes + KV_TILE - 1) / KV_TILE;
+    const int64_t units = (int64_t)n_seqs * n_kv_heads * t.row_blocks;
+    t.n_ctas = (int)(units * tiles < sms ? units * tiles : sms);
+    t.splits = tiles > 1;
+    return t;
+}
+
+cudaError_t tree_attn_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, void* out, float* lse,
+                             float* ws, cudaStream_t s) {
+    uint16_t* o = (uint16_t*)out;
+    if (head_dim == 64) return bf ? launch_all<true, 64>(p, plan, o, lse, ws, s) : launch_all<false, 64>(p, plan, o, lse, ws, s);
+    return bf ? launch_all<true, 128>(p, plan, o, lse, ws, s) : launch_all<false, 128>(p, plan, o, lse, ws, s);
+}
+
+}  // namespace jinf

@@ -21,6 +21,7 @@ STATUS_NAMES = {0: "OK", 1: "I/O error", 2: "parse error", 3: "CUDA error", 4: "
 
 # jinf_qtype values (include/jinf/quant.h)
 F32, F16, Q4_0, Q8_0, Q4_K, Q6_K = 0, 1, 2, 8, 12, 14
+BF16 = 30  # cache type of the kv_ops.h operators
 BLOCK_ELEMS = {F32: 1, F16: 1, Q4_0: 32, Q8_0: 32, Q4_K: 256, Q6_K: 256}
 BLOCK_BYTES = {F32: 4, F16: 2, Q4_0: 18, Q8_0: 34, Q4_K: 144, Q6_K: 210}
 
@@ -123,6 +124,13 @@ class NvmwTensorEntry(C.Structure):
                 ("_pad", C.c_uint8 * 3)]
 
 
+class KvStruct(C.Structure):
+    """jinf_b200_kv (include/jinf/kv_ops.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("n_seqs", C.c_int),
+                ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("max_ctx", C.c_int), ("seq_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("row_stride", C.c_int64)]
+
+
 vp, i32, i64, u64, f32, sz = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float, C.c_size_t
 
 # name -> (restype, argtypes); every function declared in include/jinf/*.h
@@ -172,6 +180,13 @@ SIGNATURES = {
     "jinf_b200_prefill_gemm": (i32, [vp, i32, i32, vp, i32, vp, vp, i32, i32, vp, vp]),
     "jinf_b200_attention_workspace_bytes": (sz, [i32, i32, i32]),
     "jinf_b200_attention_f16": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp]),
+    # kv_ops.h
+    "jinf_b200_tree_mask": (i32, [vp, i32, vp]),
+    "jinf_b200_tree_attention_workspace_bytes": (sz, [vp, i32, i32, i32]),
+    "jinf_b200_tree_attention": (i32, [vp, vp, vp, i64, i64, i32, i32, vp, vp, i32, vp, i64, f32, vp, vp]),
+    "jinf_b200_attention_mass": (i32, [vp, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp, i64, vp, f32, vp]),
+    "jinf_b200_kv_evict": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp]),
+    "jinf_b200_tree_commit": (i32, [vp, vp, vp, i32, vp, i32, vp, i32, vp, vp]),
     # gguf.h
     "jinf_gguf_open": (i32, [C.POINTER(C.POINTER(GgufFile)), C.c_char_p]),
     "jinf_gguf_close": (None, [C.POINTER(GgufFile)]),

@@ -1,0 +1,139 @@
+"""Host side of the cache operators (include/jinf/kv_ops.h): the mask of a draft tree, workspace sizes and
+the refusals, which come before any launch and need no GPU."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from jinf import _lib as L
+
+lib = L.lib
+OK, INVALID = L.JINF_OK, L.JINF_ERR_INVALID
+
+
+def tree_mask(parents):
+    n = len(parents)
+    out = np.full((max(n, 1), (n + 31) // 32 or 1), 0xDEADBEEF, dtype=np.uint32)
+    st = lib.jinf_b200_tree_mask((C.c_int32 * max(1, n))(*parents), n, out.ctypes.data_as(C.c_void_p))
+    return st, out
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 64, 200, 256])
+def test_tree_mask_is_the_ancestors(n):
+    rng = np.random.default_rng(n)
+    parents = [-1] + [int(rng.integers(-1, t)) for t in range(1, n)]
+    st, words = tree_mask(parents)
+    assert st == OK
+    for t in range(n):
+        want, u = set(), t
+        while u >= 0:
+            want.add(u)
+            u = parents[u]
+        got = {u for u in range(words.shape[1] * 32) if (int(words[t, u // 32]) >> (u % 32)) & 1}
+        assert got == want
+
+
+@pytest.mark.parametrize("parents", [[], [0], [-1, 1], [-2], [-1, 0, 5], [-1] * 257])
+def test_tree_mask_refuses(parents):
+    assert tree_mask(parents)[0] == INVALID
+
+
+def view(**kw):
+    d = dict(k=1 << 20, v=1 << 21, type=L.F16, n_seqs=2, n_kv_heads=2, head_dim=128, max_ctx=100,
+             seq_stride=2 * 100 * 128, head_stride=100 * 128, row_stride=128)
+    d.update(kw)
+    return L.KvStruct(**d)
+
+
+BAD_VIEWS = [dict(k=None), dict(v=None), dict(k=(1 << 20) + 8), dict(type=0), dict(type=12), dict(n_seqs=0),
+             dict(n_seqs=1025), dict(n_kv_heads=0), dict(head_dim=96), dict(max_ctx=0), dict(row_stride=129),
+             dict(head_stride=100 * 128 + 4), dict(seq_stride=7)]
+P = 1 << 22  # stands for a device pointer; every call below is refused before it is used
+
+
+def tree(kv, **kw):
+    d = dict(out=P, lse=P, q=P, qs=1024, qn=512, nh=4, nodes=3, n_past=P, max_past=97, mask=P, ms=0, scale=0.1, ws=P)
+    d.update(kw)
+    return lib.jinf_b200_tree_attention(d["out"], d["lse"], d["q"], d["qs"], d["qn"], d["nh"], d["nodes"],
+                                        None if kv is None else C.addressof(kv), d["n_past"], d["max_past"], d["mask"],
+                                        d["ms"], d["scale"], d["ws"], None)
+
+
+def mass(kv, **kw):
+    d = dict(mass=P, q=P, qs=1024, qn=512, nh=4, nodes=3, n_past=P, max_past=97, lse=P, mask=P, ms=0, w=None, scale=0.1)
+    d.update(kw)
+    return lib.jinf_b200_attention_mass(d["mass"], d["q"], d["qs"], d["qn"], d["nh"], d["nodes"],
+                                        None if kv is None else C.addressof(kv), d["n_past"], d["max_past"], d["lse"],
+                                        d["mask"], d["ms"], d["w"], d["scale"], None)
+
+
+QUERY = [dict(q=None), dict(q=P + 8), dict(qs=1023), dict(qn=516), dict(nh=3), dict(nh=0), dict(nodes=0),
+         dict(nodes=257), dict(n_past=None), dict(max_past=98), dict(max_past=-1), dict(ms=-1), dict(scale=0.0),
+         dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))]
+
+
+@pytest.mark.parametrize("bad", BAD_VIEWS)
+def test_bad_views_are_refused(bad):
+    kv = view(**bad)
+    assert tree(kv) == INVALID and mass(kv) == INVALID and evict(kv) == INVALID and commit(kv) == INVALID
+    assert lib.jinf_b200_tree_attention_workspace_bytes(C.addressof(kv), 4, 3, 97) == 0
+
+
+@pytest.mark.parametrize("bad", QUERY + [dict(out=None), dict(out=P + 4), dict(ws=None), dict(ws=P + 8)])
+def test_tree_attention_refuses(bad):
+    assert tree(view(), **bad) == INVALID
+    assert tree(None) == INVALID
+
+
+@pytest.mark.parametrize("bad", QUERY + [dict(mass=None), dict(lse=None)])
+def test_attention_mass_refuses(bad):
+    assert mass(view(), **bad) == INVALID
+    assert mass(None) == INVALID
+
+
+def evict(kv, out=None, **kw):
+    d = dict(mass=P, mass_out=None, n_rows=P, ids=P, n_out=None, keep=10, sink=2, recent=3)
+    d.update(kw)
+    return lib.jinf_b200_kv_evict(None if kv is None else C.addressof(kv), None if out is None else C.addressof(out),
+                                  d["mass"], d["mass_out"], d["n_rows"], d["ids"], d["n_out"], d["keep"], d["sink"],
+                                  d["recent"], None)
+
+
+@pytest.mark.parametrize("bad", [dict(mass=None), dict(n_rows=None), dict(ids=None), dict(keep=0), dict(keep=101),
+                                 dict(sink=-1), dict(recent=-1), dict(sink=8), dict(recent=11),
+                                 dict(sink=2 ** 31 - 1, recent=2 ** 31 - 1), dict(n_out=P),
+                                 dict(mass_out=2 * P)])  # in place, the mass too
+def test_kv_evict_refuses(bad):
+    assert evict(view(), **bad) == INVALID
+    assert evict(None) == INVALID
+
+
+@pytest.mark.parametrize("bad", [dict(type=L.BF16), dict(n_seqs=1), dict(n_kv_heads=1), dict(head_dim=64),
+                                 dict(max_ctx=9), dict(k=1 << 20), dict(v=1 << 21),
+                                 dict(k=1 << 20, v=1 << 21, row_stride=256)])
+def test_kv_evict_refuses_outputs_that_do_not_match(bad):
+    d = dict(k=1 << 24, v=1 << 25)
+    d.update(bad)
+    assert evict(view(), view(**d)) == INVALID
+    assert evict(view(), view(k=1 << 24, v=1 << 25), mass_out=P) == INVALID  # another cache, the same mass
+
+
+def commit(kv, **kw):
+    d = dict(mass=None, n_past=P, max_past=90, acc=P, stride=4, n_acc=P, nodes=10, n_out=None)
+    d.update(kw)
+    return lib.jinf_b200_tree_commit(None if kv is None else C.addressof(kv), d["mass"], d["n_past"], d["max_past"],
+                                     d["acc"], d["stride"], d["n_acc"], d["nodes"], d["n_out"], None)
+
+
+@pytest.mark.parametrize("bad", [dict(n_past=None), dict(acc=None), dict(n_acc=None), dict(max_past=91),
+                                 dict(max_past=-1), dict(stride=0), dict(nodes=0), dict(nodes=257), dict(n_out=P)])
+def test_tree_commit_refuses(bad):
+    assert commit(view(), **bad) == INVALID
+    assert commit(None) == INVALID
+
+
+def test_workspace_is_bounded_by_the_device_not_by_the_context():
+    kv = view(max_ctx=1 << 20, seq_stride=1 << 28, head_stride=1 << 27)
+    small = lib.jinf_b200_tree_attention_workspace_bytes(C.addressof(kv), 4, 3, 97)
+    large = lib.jinf_b200_tree_attention_workspace_bytes(C.addressof(kv), 4, 3, (1 << 20) - 3)
+    assert 0 < small <= large < 64 << 20
