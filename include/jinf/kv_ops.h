@@ -31,6 +31,7 @@ extern "C" {
 #define JINF_B200_BF16 30
 
 #define JINF_TREE_MAX_NODES 256
+#define JINF_TREE_MAX_GROUP 64  // query heads per kv head
 #define JINF_KV_MAX_SEQS 1024
 
 // K and V rows of n_seqs sequences (or layers, or both): row r of kv head h of sequence s is the

@@ -35,7 +35,12 @@ static bool kv_ok(const jinf_b200_kv* kv) {
 static bool tree_shape_ok(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past) {
     return kv_ok(kv) && n_heads >= 1 && n_heads % kv->n_kv_heads == 0 && n_nodes >= 1 &&
            n_nodes <= JINF_TREE_MAX_NODES && max_past >= 0 && max_past <= kv->max_ctx - n_nodes &&
-           n_heads / kv->n_kv_heads <= 1024;
+           n_heads / kv->n_kv_heads <= JINF_TREE_MAX_GROUP;
+}
+
+static TreePlan plan_of(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past) {
+    return tree_plan(kv->n_seqs, kv->n_kv_heads, n_nodes * (n_heads / kv->n_kv_heads), n_nodes, max_past, kv_device_sms(),
+                     tree_mma_fits(kv));
 }
 
 static void tree_params(TreeParams* p, const void* q, int64_t q_seq, int64_t q_node, int n_heads, int n_nodes,
@@ -85,9 +90,7 @@ extern "C" jinf_status jinf_b200_tree_mask(const int32_t* parents, int n_nodes, 
 extern "C" size_t jinf_b200_tree_attention_workspace_bytes(const jinf_b200_kv* kv, int n_heads, int n_nodes,
                                                            int max_past) {
     if (!tree_shape_ok(kv, n_heads, n_nodes, max_past)) return 0;
-    const TreePlan plan = tree_plan(kv->n_seqs, kv->n_kv_heads, n_nodes * (n_heads / kv->n_kv_heads), n_nodes, max_past,
-                                    kv->head_dim, kv_device_sms());
-    return sizeof(float) * tree_workspace_floats(plan.block_rows, kv->head_dim, plan.n_ctas);
+    return tree_workspace_bytes(plan_of(kv, n_heads, n_nodes, max_past), kv->head_dim);
 }
 
 extern "C" jinf_status jinf_b200_tree_attention(void* out, float* lse, const void* q, int64_t q_seq_stride,
@@ -100,10 +103,10 @@ extern "C" jinf_status jinf_b200_tree_attention(void* out, float* lse, const voi
         return JINF_ERR_INVALID;
     TreeParams p;
     tree_params(&p, q, q_seq_stride, q_node_stride, n_heads, n_nodes, kv, n_past, max_past, mask, mask_seq_stride, scale);
-    const TreePlan plan = tree_plan(p.n_seqs, p.n_kv_heads, p.n_rows, n_nodes, max_past, kv->head_dim, kv_device_sms());
+    const TreePlan plan = plan_of(kv, n_heads, n_nodes, max_past);
     p.row_blocks = plan.row_blocks;
     p.block_rows = plan.block_rows;
-    return tree_attn_launch(p, plan, kv->type == JINF_B200_BF16, kv->head_dim, out, lse, (float*)workspace, stream) ==
+    return tree_attn_launch(p, plan, kv->type == JINF_B200_BF16, kv->head_dim, out, lse, workspace, stream) ==
                    cudaSuccess
                ? JINF_OK
                : JINF_ERR_CUDA;

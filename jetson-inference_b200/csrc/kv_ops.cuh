@@ -86,86 +86,108 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)_
 
 // ---- division of the work ----
 //
-// A unit is one (sequence, kv head, row block); it has ceil((n_past + n_nodes) / KV_TILE) key
-// tiles. The tiles of all units, in order, are dealt to the CTAs in equal contiguous shares, so
-// the division is even whatever the sequences' lengths, and is computed on the device from them.
+// A unit is one (sequence, kv head); it has ceil((n_past + n_nodes) / KV_TILE) key tiles. The tiles
+// of all units, in order, are dealt to groups of row_blocks CTAs in equal contiguous shares, so the
+// division is even whatever the sequences' lengths, and is computed on the device from them. The
+// CTAs of a group take one block of query rows each over the same tiles at about the same time, so
+// that DRAM delivers K and V once and L2 the other times.
 constexpr int KV_TILE = 128;
 
-__device__ __forceinline__ int seq_tiles(const TreeParams& p, int seq) {
-    return (clamped_past(p, seq) + p.n_nodes + KV_TILE - 1) / KV_TILE;
+__device__ __forceinline__ int seq_tiles(const TreeParams& p, int past) {
+    return (past + p.n_nodes + KV_TILE - 1) / KV_TILE;
+}
+// Groups that get a share: none is empty, so the parts of a unit are those of consecutive groups.
+__device__ __forceinline__ int share_count(int64_t total, int n) { return (int)min((int64_t)n, total); }
+__device__ __forceinline__ int64_t share_start(int64_t total, int g, int n) { return total * g / n; }
+// The group whose share holds tile t.
+__device__ __forceinline__ int share_owner(int64_t total, int64_t t, int n) {
+    int g = (int)((t * n) / total);
+    while (g + 1 < n && share_start(total, g + 1, n) <= t) ++g;
+    while (g > 0 && share_start(total, g, n) > t) --g;
+    return g;
 }
 
-// prefix[s] = tiles of one (kv head, row block) over the sequences before s, s <= n_seqs; all
-// threads of the CTA call it. `prefix` holds n_seqs + 1 ints of shared memory.
-__device__ __forceinline__ void tile_prefix(const TreeParams& p, int* prefix) {
-    if (threadIdx.x < 32) {
-        int base = 0;
-        for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
-            const int s = s0 + (int)threadIdx.x;
-            int t = s < p.n_seqs ? seq_tiles(p, s) : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int x = __shfl_up_sync(JINF_FULL_MASK, t, o);
-                if ((int)threadIdx.x >= o) t += x;
-            }
-            if (s < p.n_seqs) prefix[s + 1] = base + t;
-            base += __shfl_sync(JINF_FULL_MASK, t, 31);
-        }
-        if (threadIdx.x == 0) prefix[0] = 0;
-    }
-    __syncthreads();
-}
-
-struct Unit {
-    int seq, head, block;
-    int64_t first;  // the unit's first tile, in the numbering over all units
-    int tiles;
+// A part of a unit: tiles t0..t1 - 1 of its `tiles`.
+struct Segment {
+    int seq, head, past, tiles, t0, t1;
 };
+// A group's share, walked segment by segment.
+struct Share {
+    int64_t left;  // tiles not yet handed out
+    int seq, head, tile;
 
-// The unit that holds global tile `t` (units ordered by sequence, head, block).
-__device__ __forceinline__ Unit unit_of(const TreeParams& p, const int* prefix, int64_t t) {
-    const int per = p.n_kv_heads * p.row_blocks;
-    int lo = 0, hi = p.n_seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if ((int64_t)prefix[mid] * per <= t) lo = mid; else hi = mid - 1;
+    __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
+        if (left <= 0) return false;
+        s.seq = seq;
+        s.head = head;
+        s.past = clamped_past(p, seq);
+        s.tiles = seq_tiles(p, s.past);
+        s.t0 = tile;
+        s.t1 = (int)min((int64_t)s.tiles, tile + left);
+        left -= s.t1 - s.t0;
+        tile = 0;
+        if (++head == p.n_kv_heads) {
+            head = 0;
+            ++seq;
+        }
+        return true;
     }
-    Unit u;
-    u.seq = lo;
-    u.tiles = prefix[lo + 1] - prefix[lo];
-    const int64_t in_seq = t - (int64_t)prefix[lo] * per;
-    const int hb = (int)(in_seq / u.tiles);
-    u.head = hb / p.row_blocks;
-    u.block = hb % p.row_blocks;
-    u.first = t - in_seq + (int64_t)hb * u.tiles;
-    return u;
-}
-
-// CTAs that get a share: none is empty, so the parts of a unit are those of consecutive CTAs.
-__device__ __forceinline__ int share_count(int64_t total, int n_ctas) { return (int)min((int64_t)n_ctas, total); }
-__device__ __forceinline__ int64_t share_start(int64_t total, int cta, int n_ctas) { return total * cta / n_ctas; }
-// The CTA whose share holds tile t.
-__device__ __forceinline__ int share_owner(int64_t total, int64_t t, int n_ctas) {
-    int c = (int)((t * n_ctas) / total);
-    while (c + 1 < n_ctas && share_start(total, c + 1, n_ctas) <= t) ++c;
-    while (c > 0 && share_start(total, c, n_ctas) > t) --c;
-    return c;
+};
+// Group g's share of n groups, found by one warp (all its lanes get it).
+__device__ __forceinline__ Share share_begin(const TreeParams& p, int g, int n) {
+    const int lane = threadIdx.x & 31;
+    int64_t sum = 0;
+    for (int s = lane; s < p.n_seqs; s += 32) sum += seq_tiles(p, clamped_past(p, s));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(JINF_FULL_MASK, sum, o);
+    const int64_t total = sum * p.n_kv_heads;
+    n = share_count(total, n);
+    Share sh{0, 0, 0, 0};
+    if (g >= n) return sh;
+    const int64_t begin = share_start(total, g, n);
+    sh.left = share_start(total, g + 1, n) - begin;
+    int64_t base = 0;  // tiles of one head over the sequences before this round's
+    for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
+        const int s = s0 + lane, t = s < p.n_seqs ? seq_tiles(p, clamped_past(p, s)) : 0;
+        int64_t upto = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(JINF_FULL_MASK, upto, o);
+            if (lane >= o) upto += x;
+        }
+        upto += base;
+        const uint32_t has = __ballot_sync(JINF_FULL_MASK, upto * p.n_kv_heads > begin);
+        if (has) {
+            const int at = __ffs(has) - 1;
+            const int tiles = __shfl_sync(JINF_FULL_MASK, t, at);
+            const int64_t in_seq = begin - (__shfl_sync(JINF_FULL_MASK, upto, at) - tiles) * p.n_kv_heads;
+            sh.seq = s0 + at;
+            sh.head = (int)(in_seq / tiles);
+            sh.tile = (int)(in_seq % tiles);
+            return sh;
+        }
+        base = __shfl_sync(JINF_FULL_MASK, upto, 31);
+    }
+    return sh;
 }
 
 int kv_device_sms();  // SMs of the current device (cached per device)
 
 // ---- launches (return a cudaError_t; arguments already checked) ----
 
-// fp32 scratch of a tree attention: partial rows of the units that several CTAs share. CTA c's
-// two slots (a unit begun by an earlier CTA; one it hands on) hold block_rows rows each.
-size_t tree_workspace_floats(int block_rows, int head_dim, int n_ctas);
 struct TreePlan {
-    int row_blocks, block_rows, n_ctas;
-    bool splits;  // some unit may be shared by several CTAs
+    int row_blocks, block_rows;
+    int n_groups;  // grid: n_groups * row_blocks CTAs
+    bool mma;      // k_tree_mma, else k_tree_rows
+    bool splits;   // some unit may be shared by several groups
 };
-TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int head_dim, int sms);
+TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int sms,
+                   bool mma_fits);
+size_t tree_workspace_bytes(const TreePlan& plan, int head_dim);
+// k_tree_mma's tensor maps describe this cache (their strides are below 2^40 bytes and not 0)
+bool tree_mma_fits(const jinf_b200_kv* kv);
 cudaError_t tree_attn_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, void* out, float* lse,
-                             float* ws, cudaStream_t s);
+                             void* ws, cudaStream_t s);
 
 cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, const float* lse, const float* weight,
                              float* mass, cudaStream_t s);

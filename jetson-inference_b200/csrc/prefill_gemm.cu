@@ -28,8 +28,8 @@
 #include "common.cuh"
 #include "q4m.cuh"
 #include "prefill.h"
+#include "umma.cuh"
 
-#include <cuda.h>
 #include <cuda_fp16.h>
 
 namespace jinf {
@@ -41,7 +41,6 @@ constexpr int PG_A_BYTES = 2 * PG_ATOM;               // 128 rows x 128 columns 
 constexpr int PG_B_BYTES = 2 * PG_ATOM;               // 128 tokens x 128 columns fp16
 constexpr int PG_RAW_BYTES = 4 * Q4M_UNIT;            // four tile pairs of one group
 constexpr int PG_DQ_THREADS = 448;                    // warps 2..15
-constexpr unsigned long long PG_SPIN = 1ull << 22;    // polls of a wait before it gives up
 
 // shared memory offsets from the 1024-aligned base
 constexpr int PG_OFF_A = 0;
@@ -50,68 +49,7 @@ constexpr int PG_OFF_RAW = PG_OFF_B + PG_STAGES * PG_B_BYTES;
 constexpr int PG_OFF_BAR = PG_OFF_RAW + PG_STAGES * PG_RAW_BYTES;
 constexpr int PG_SMEM = PG_OFF_BAR + 256 + 1024;      // + barriers + alignment slack
 
-__device__ __forceinline__ uint32_t su32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mb_init(uint32_t b, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mb_expect(uint32_t b, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mb_arrive(uint32_t b) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
-}
-// Bounded wait for phase `parity` of the mbarrier; false when it ran out.
-__device__ __forceinline__ bool mb_wait(uint32_t b, uint32_t parity) {
-    for (unsigned long long it = 0; it < PG_SPIN; ++it) {
-        uint32_t ok;
-        asm volatile(
-            "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-            : "=r"(ok)
-            : "r"(b), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if (it > 64) __nanosleep(64);
-    }
-    return false;
-}
-
-// raw bytes global -> shared on an mbarrier (16-byte aligned, a multiple of 16 bytes)
-__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
-// one box of the 2-D tensor map (x: column, y: token) into shared memory, this GPU's own memory
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-            dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-
-// UMMA shared-memory descriptor of a K-major, 128B-swizzled operand: start address, leading
-// byte offset 16 (unused with this swizzle), stride byte offset 1024 (eight 128-byte rows),
-// descriptor version 1, swizzle mode 2 (128B).
-__device__ __forceinline__ uint64_t umma_desc(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// Instruction descriptor of kind::f16: f32 accumulator, f16 A and B, both K-major, N 128, M 128.
-constexpr uint32_t PG_IDESC = (1u << 4) | (0u << 7) | (0u << 10) | ((uint32_t)(PG_BN >> 3) << 17) |
-                              ((uint32_t)(PG_BM >> 4) << 24);
-
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
-    asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(PG_IDESC), "r"(accumulate)
-        : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
+constexpr uint32_t PG_IDESC = umma_idesc(false, PG_BM, PG_BN, false);
 
 // (q - 8) * d for the four bytes of a word, low nibbles (tile A row) or high nibbles (tile B
 // row): two half2 in k order. 0x6400 | q is the fp16 1024 + q, so subtracting 1032 gives q - 8
@@ -236,7 +174,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1)
 #pragma unroll
                 for (int kk = 0; kk < PG_BK / 16; ++kk) {
                     const uint32_t off = (uint32_t)((kk >> 2) * PG_ATOM + (kk & 3) * 32);
-                    umma_f16(tmem, umma_desc(a0 + off), umma_desc(bb0 + off), (kt | kk) ? 1u : 0u);
+                    umma_ss(tmem, umma_desc(a0 + off), umma_desc(bb0 + off), PG_IDESC, (kt | kk) ? 1u : 0u);
                 }
                 umma_commit(b_empty + 8 * s);
                 ++issued;
@@ -274,17 +212,8 @@ __global__ void __launch_bounds__(PG_THREADS, 1)
                 for (int c0 = 0; c0 < PG_BN; c0 += 32) {
                     uint32_t v[32];
                     const uint32_t taddr = tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)c0;
-                    asm volatile(
-                        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
-                        "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
-                        "[%32];"
-                        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-                          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]),
-                          "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
-                          "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]),
-                          "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-                        : "r"(taddr));
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    tmem_ld32(taddr, v);
+                    tmem_wait_ld();
                     if (row < rows) {
 #pragma unroll
                         for (int jj = 0; jj < 32; ++jj) {
@@ -315,22 +244,6 @@ __global__ void __launch_bounds__(PG_THREADS, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 128;" ::"r"(tmem) : "memory");
     }
-}
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = (EncodeTiledFn)p;
-    }
-    return fn;
 }
 
 }  // namespace

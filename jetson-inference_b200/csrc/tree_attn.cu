@@ -12,10 +12,9 @@
 // by tile (kv_ops.cuh); a CTA's eight warps join their (m, l, O) in shared memory, and
 // k_tree_merge joins what several CTAs hold of one unit.
 #include "kv_ops.cuh"
+#include "tree_part.cuh"
 
 #include <math.h>
-
-#include <type_traits>
 
 namespace jinf {
 namespace {
@@ -28,47 +27,41 @@ static_assert(TW * WKEYS == KV_TILE, "a tile is one chunk of each warp");
 template <int HD, int MT>
 struct RowsSmem {
     static constexpr int RING = TW * TS * 2 * WKEYS * HD * 2;     // bytes
-    static constexpr int JOIN = TW * 16 * MT * (HD + 2) * 4;      // the warps' (O, m, l) at the end of a unit
+    static constexpr int JOIN = TW * 16 * MT * (HD + 6) * 4;      // the warps' (O, m, l) at the end of a unit
     static constexpr int Q = 16 * MT * HD * 2;
     static constexpr int UNION = RING > JOIN ? RING : JOIN;
-    static constexpr int TOTAL = UNION + Q;                       // + prefix
+    static constexpr int TOTAL = UNION + Q;
 };
-
-// The partial rows of CTA c's slot: [block_rows][HD] O (unnormalised, of scale e^-m), then
-// [block_rows] m (of the unscaled scores) and [block_rows] l; slots start on 16 bytes.
-__host__ __device__ __forceinline__ size_t slot_floats(int block_rows, int hd) {
-    return ((size_t)block_rows * (hd + 2) + 3) & ~(size_t)3;
-}
 
 template <bool BF, int HD, int MT>
 __global__ void __launch_bounds__(TW * 32, 1)
-    k_tree_rows(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, float* __restrict__ ws) {
+    k_tree_rows(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, float* __restrict__ parts) {
     using SM = RowsSmem<HD, MT>;
     constexpr int CH = HD / 8;       // 16-byte chunks of a row
     constexpr int ROWB = HD * 2;     // bytes of a row
     constexpr int KS = HD / 16;      // k steps of q.k
     constexpr int NT = HD / 8;       // column tiles of O
+    constexpr int JP = HD + 4;       // floats between two joined rows (conflict-free down the rows)
     extern __shared__ __align__(128) uint8_t sm[];
     float* join = reinterpret_cast<float*>(sm);
     uint8_t* sq = sm + SM::UNION;
-    int* prefix = reinterpret_cast<int*>(sm + SM::TOTAL);
+    __shared__ Share s_share;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = smem_u32(sm) + warp * (TS * 2 * WKEYS * ROWB);
 
-    tile_prefix(p, prefix);
-    const int64_t total = (int64_t)prefix[p.n_seqs] * p.n_kv_heads * p.row_blocks;
-    const int n_ctas = share_count(total, gridDim.x);
-    if ((int)blockIdx.x >= n_ctas) return;
-    const int64_t begin = share_start(total, blockIdx.x, n_ctas), end = share_start(total, blockIdx.x + 1, n_ctas);
+    const int block = blockIdx.x % p.row_blocks, group = blockIdx.x / p.row_blocks;
+    const int row0 = block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
+    if (warp == 0) {
+        const Share sh = share_begin(p, group, gridDim.x / p.row_blocks);
+        if (lane == 0) s_share = sh;
+    }
+    __syncthreads();
+    Share share = s_share;
     const float c2 = p.scale * LOG2E;
 
-    for (int64_t at = begin; at < end;) {
-        const Unit u = unit_of(p, prefix, at);
-        const int t0 = (int)(at - u.first);
-        const int t1 = (int)min((int64_t)u.tiles, end - u.first);
-        at = u.first + t1;
-        const int past = clamped_past(p, u.seq), n_keys = past + p.n_nodes;
-        const int row0 = u.block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
+    for (Segment u; share.next(p, u);) {
+        const int t0 = u.t0, t1 = u.t1;
+        const int past = u.past, n_keys = past + p.n_nodes;
         const uint32_t* mask = p.mask ? p.mask + u.seq * p.mask_seq : nullptr;
         const int64_t kvo = (u.seq * p.kv_seq + u.head * p.kv_head) * 2;
 
@@ -255,7 +248,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
         __syncthreads();  // every warp is done with its ring and with the queries
 
         // join the warps
-        float* jm = join + TW * 16 * MT * HD;
+        float* jm = join + TW * 16 * MT * JP;
         float* jl = jm + TW * 16 * MT;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -271,14 +264,14 @@ __global__ void __launch_bounds__(TW * 32, 1)
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    *reinterpret_cast<float2*>(join + ((size_t)warp * 16 * MT + r) * HD + 8 * n + 2 * (lane & 3)) =
+                    *reinterpret_cast<float2*>(join + (warp * 16 * MT + r) * JP + 8 * n + 2 * (lane & 3)) =
                         make_float2(o[mt][n][2 * h], o[mt][n][2 * h + 1]);
             }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == u.tiles;
-        float* part = ws + ((size_t)blockIdx.x * 2 + (t0 == 0 ? 1 : 0)) * slot_floats(p.block_rows, HD);
+        float* part = parts + ((size_t)blockIdx.x * 2 + (t0 == 0 ? 1 : 0)) * part_floats(p.block_rows, HD);
         for (int i = tid; i < rows * (HD / 4); i += TW * 32) {
-            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            const int r = i % rows, d = (i / rows) * 4;
             float M = -INFINITY;
 #pragma unroll
             for (int w = 0; w < TW; ++w) M = fmaxf(M, jm[w * 16 * MT + r]);
@@ -288,7 +281,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
 #pragma unroll
             for (int w = 0; w < TW; ++w) {
                 const float f = exp2f((jm[w * 16 * MT + r] - base) * c2);
-                const float4 x = *reinterpret_cast<const float4*>(join + ((size_t)w * 16 * MT + r) * HD + d);
+                const float4 x = *reinterpret_cast<const float4*>(join + (w * 16 * MT + r) * JP + d);
                 L = fmaf(jl[w * 16 * MT + r], f, L);
                 a.x = fmaf(x.x, f, a.x);
                 a.y = fmaf(x.y, f, a.y);
@@ -303,7 +296,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
                 *reinterpret_cast<uint2*>(out + orow * HD + d) = w2;
                 if (lse && d == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
             } else {
-                *reinterpret_cast<float4*>(part + (size_t)r * HD + d) = a;
+                *reinterpret_cast<float4*>(part + ((size_t)(d / 4) * p.block_rows + r) * 4) = a;
                 if (d == 0) {
                     part[(size_t)p.block_rows * HD + r] = M;
                     part[(size_t)p.block_rows * (HD + 1) + r] = L;
@@ -315,155 +308,152 @@ __global__ void __launch_bounds__(TW * 32, 1)
     pdl_trigger();
 }
 
-constexpr int MERGE_WARPS = 8;
+constexpr int MERGE_THREADS = 256;
 
-// Joins the parts of the units that several CTAs share: one warp per row, each part's O scaled by
-// e^(m_part - m) and added in the order of the CTAs.
+// Joins the parts of the units that several groups share. blockIdx.x: (sequence, kv head, row
+// block); a thread owns four columns of one row and adds the parts in the groups' order, each
+// scaled by e^(m_part - m), eight parts' loads in flight.
 template <bool BF, int HD>
-__global__ void __launch_bounds__(MERGE_WARPS * 32)
-    k_tree_merge(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, const float* __restrict__ ws,
-                 int n_ctas) {
-    extern __shared__ int prefix[];
-    constexpr int V = HD / 32;  // values of a lane
-    tile_prefix(p, prefix);
-    const int64_t total = (int64_t)prefix[p.n_seqs] * p.n_kv_heads * p.row_blocks;
-    n_ctas = share_count(total, n_ctas);
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * MERGE_WARPS + (threadIdx.x >> 5);  // over (seq, kv head, row)
-    const bool ok = row < (int64_t)p.n_seqs * p.n_kv_heads * p.n_rows;
-    int c0 = 0, c1 = 0, r = 0, rr = 0, seq = 0, head = 0;
-    int64_t first = 0;
-    if (ok) {
-        rr = (int)(row % p.n_rows);
-        const int64_t sh = row / p.n_rows;
-        head = (int)(sh % p.n_kv_heads);
-        seq = (int)(sh / p.n_kv_heads);
-        const int tiles = prefix[seq + 1] - prefix[seq], block = rr / p.block_rows;
-        r = rr % p.block_rows;
-        first = ((int64_t)prefix[seq] * p.n_kv_heads + (int64_t)head * tiles) * p.row_blocks + (int64_t)block * tiles;
-        c0 = share_owner(total, first, n_ctas);
-        c1 = share_owner(total, first + tiles - 1, n_ctas);
+__global__ void __launch_bounds__(MERGE_THREADS)
+    k_tree_merge(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, const float* __restrict__ parts,
+                 int n_groups) {
+    __shared__ int64_t s_before, s_all;  // tiles of one kv head: of the sequences before this one, and of all
+    const int block = blockIdx.x % p.row_blocks, sh = blockIdx.x / p.row_blocks;
+    const int head = sh % p.n_kv_heads, seq = sh / p.n_kv_heads;
+    if (threadIdx.x < 32) {
+        int64_t before = 0, all = 0;
+        for (int s = threadIdx.x; s < p.n_seqs; s += 32) {
+            const int t = seq_tiles(p, clamped_past(p, s));
+            all += t;
+            if (s < seq) before += t;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            before += __shfl_xor_sync(JINF_FULL_MASK, before, o);
+            all += __shfl_xor_sync(JINF_FULL_MASK, all, o);
+        }
+        if (threadIdx.x == 0) {
+            s_before = before;
+            s_all = all;
+        }
     }
+    __syncthreads();
+    const int64_t total = s_all * p.n_kv_heads;
+    n_groups = share_count(total, n_groups);
+    const int tiles = seq_tiles(p, clamped_past(p, seq));
+    const int64_t first = s_before * p.n_kv_heads + (int64_t)head * tiles;
+    const int g0 = share_owner(total, first, n_groups), g1 = share_owner(total, first + tiles - 1, n_groups);
+    const int row0 = block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
+    const int i = blockIdx.y * MERGE_THREADS + threadIdx.x;
     pdl_wait();  // the parts below are the previous kernel's
-    if (c0 == c1) return;
-    const size_t sf = slot_floats(p.block_rows, HD);
+    if (g0 == g1 || i >= rows * (HD / 4)) return;
+    const int r = i % rows, d4 = i / rows;
+    const size_t pf = part_floats(p.block_rows, HD);
     const float c2 = p.scale * LOG2E;
-    float M = -INFINITY, L = 0.f, a[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) a[v] = 0.f;
+    float M = -INFINITY, L = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int B = 8;
-    for (int cb = c0; cb <= c1; cb += B) {
-        float pm[B], pl[B], po[B][V];
+    for (int gb = g0; gb <= g1; gb += B) {
+        float pm[B], pl[B];
+        float4 po[B];
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const int c = cb + i;
-            pm[i] = -INFINITY;
-            pl[i] = 0.f;
-            if (c <= c1) {
-                // the CTA that begins the unit kept it in its second slot, the others in their first
-                const float* part = ws + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * sf;
-                pm[i] = __ldcg(part + (size_t)p.block_rows * HD + r);
-                pl[i] = __ldcg(part + (size_t)p.block_rows * (HD + 1) + r);
-                if constexpr (V == 4) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4*>(part + (size_t)r * HD) + lane);
-                    po[i][0] = x.x; po[i][1] = x.y; po[i][2] = x.z; po[i][3] = x.w;
-                } else {
-                    const float2 x = __ldcg(reinterpret_cast<const float2*>(part + (size_t)r * HD) + lane);
-                    po[i][0] = x.x; po[i][1] = x.y;
-                }
-            } else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) po[i][v] = 0.f;
+        for (int k = 0; k < B; ++k) {
+            const int g = gb + k;
+            pm[k] = -INFINITY;
+            pl[k] = 0.f;
+            po[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (g <= g1) {
+                // the group that begins the unit kept it in its second slot, the others in their first
+                const float* part = parts + (((size_t)g * p.row_blocks + block) * 2 + (g == g0 ? 1 : 0)) * pf;
+                pm[k] = __ldcg(part + (size_t)p.block_rows * HD + r);
+                pl[k] = __ldcg(part + (size_t)p.block_rows * (HD + 1) + r);
+                po[k] = __ldcg(reinterpret_cast<const float4*>(part) + (size_t)d4 * p.block_rows + r);
             }
         }
         float mn = M;
 #pragma unroll
-        for (int i = 0; i < B; ++i) mn = fmaxf(mn, pm[i]);
+        for (int k = 0; k < B; ++k) mn = fmaxf(mn, pm[k]);
         const float base = mn == -INFINITY ? 0.f : mn;
         const float corr = exp2f((M - base) * c2);
         M = mn;
         L *= corr;
+        a.x *= corr; a.y *= corr; a.z *= corr; a.w *= corr;
 #pragma unroll
-        for (int v = 0; v < V; ++v) a[v] *= corr;
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            const float f = exp2f((pm[i] - base) * c2);
-            L = fmaf(pl[i], f, L);
-#pragma unroll
-            for (int v = 0; v < V; ++v) a[v] = fmaf(po[i][v], f, a[v]);
+        for (int k = 0; k < B; ++k) {
+            const float f = exp2f((pm[k] - base) * c2);
+            L = fmaf(pl[k], f, L);
+            a.x = fmaf(po[k].x, f, a.x);
+            a.y = fmaf(po[k].y, f, a.y);
+            a.z = fmaf(po[k].z, f, a.z);
+            a.w = fmaf(po[k].w, f, a.w);
         }
     }
+    const int rr = row0 + r;
     const size_t orow = ((size_t)seq * p.n_nodes + rr / p.group) * p.n_heads + head * p.group + rr % p.group;
     const float inv = L > 0.f ? 1.f / L : L == 0.f ? 1.f : L;
-    if constexpr (V == 4)
-        *reinterpret_cast<uint2*>(out + orow * HD + lane * 4) =
-            make_uint2(pack2<BF>(a[0] * inv, a[1] * inv), pack2<BF>(a[2] * inv, a[3] * inv));
-    else
-        *reinterpret_cast<uint32_t*>(out + orow * HD + lane * 2) = pack2<BF>(a[0] * inv, a[1] * inv);
-    if (lse && lane == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
+    *reinterpret_cast<uint2*>(out + orow * HD + d4 * 4) =
+        make_uint2(pack2<BF>(a.x * inv, a.y * inv), pack2<BF>(a.z * inv, a.w * inv));
+    if (lse && d4 == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
 }
 
-template <typename K>
-cudaError_t launch(K kernel, dim3 grid, int threads, size_t smem, bool pdl, cudaStream_t s, const TreeParams& p,
-                   uint16_t* out, float* lse, float* ws, int n_ctas) {
+template <bool BF, int HD, int MT>
+cudaError_t launch_rows(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* parts, cudaStream_t s) {
+    constexpr int smem = RowsSmem<HD, MT>::TOTAL;
+    const cudaError_t e = cudaFuncSetAttribute(k_tree_rows<BF, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    k_tree_rows<BF, HD, MT><<<plan.n_groups * plan.row_blocks, TW * 32, smem, s>>>(p, out, lse, parts);
+    return cudaGetLastError();
+}
+
+template <bool BF, int HD>
+cudaError_t launch_all(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* parts, int* err,
+                       cudaStream_t s) {
+    const cudaError_t e = plan.mma                 ? tree_mma_launch(p, plan, BF, HD, out, lse, parts, err, s)
+                          : plan.block_rows <= 16 ? launch_rows<BF, HD, 1>(p, plan, out, lse, parts, s)
+                                                  : launch_rows<BF, HD, 2>(p, plan, out, lse, parts, s);
+    if (e != cudaSuccess || !plan.splits) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3((unsigned)(p.n_seqs * p.n_kv_heads * p.row_blocks),
+                       (unsigned)((p.block_rows * (HD / 4) + MERGE_THREADS - 1) / MERGE_THREADS));
+    cfg.blockDim = dim3(MERGE_THREADS);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-    if constexpr (std::is_invocable_v<K, const TreeParams, uint16_t*, float*, const float*, int>)
-        return cudaLaunchKernelEx(&cfg, kernel, p, out, lse, (const float*)ws, n_ctas);
-    else
-        return cudaLaunchKernelEx(&cfg, kernel, p, out, lse, ws);
-}
-
-template <bool BF, int HD, int MT>
-cudaError_t launch_rows(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* ws, cudaStream_t s) {
-    const size_t smem = RowsSmem<HD, MT>::TOTAL + (size_t)(JINF_KV_MAX_SEQS + 1) * sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(k_tree_rows<BF, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    return launch(k_tree_rows<BF, HD, MT>, dim3(plan.n_ctas), TW * 32, smem, false, s, p, out, lse, ws, plan.n_ctas);
-}
-
-template <bool BF, int HD>
-cudaError_t launch_all(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* ws, cudaStream_t s) {
-    cudaError_t e = plan.block_rows <= 16 ? launch_rows<BF, HD, 1>(p, plan, out, lse, ws, s)
-                                          : launch_rows<BF, HD, 2>(p, plan, out, lse, ws, s);
-    if (e != cudaSuccess || !plan.splits) return e;
-    const int64_t rows = (int64_t)p.n_seqs * p.n_kv_heads * p.n_rows;
-    return launch(k_tree_merge<BF, HD>, dim3((unsigned)((rows + MERGE_WARPS - 1) / MERGE_WARPS)), MERGE_WARPS * 32,
-                  (size_t)(p.n_seqs + 1) * sizeof(int), true, s, p, out, lse, ws, plan.n_ctas);
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_tree_merge<BF, HD>, p, out, lse, (const float*)parts, plan.n_groups);
 }
 
 }  // namespace
 
-size_t tree_workspace_floats(int block_rows, int head_dim, int n_ctas) {
-    return (size_t)n_ctas * 2 * slot_floats(block_rows, head_dim);
+size_t tree_workspace_bytes(const TreePlan& plan, int head_dim) {
+    return TREE_WS_HEAD + sizeof(float) * (size_t)plan.n_groups * plan.row_blocks * 2 * part_floats(plan.block_rows, head_dim);
 }
 
-TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int head_dim, int sms) {
-    (void)head_dim;
+TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int sms,
+                   bool mma_fits) {
     TreePlan t;
-    t.row_blocks = (n_rows + 31) / 32;
+    t.mma = n_rows > 16 && mma_fits;
+    const int most = t.mma ? 256 : 32;
+    t.row_blocks = (n_rows + most - 1) / most;
     t.block_rows = (n_rows + t.row_blocks - 1) / t.row_blocks;
     t.row_blocks = (n_rows + t.block_rows - 1) / t.block_rows;
-    const int64_t tiles = (max_past + n_nodes + KV_TILE - 1) / KV_TILE;
-    const int64_t units = (int64_t)n_seqs * n_kv_heads * t.row_blocks;
-    t.n_ctas = (int)(units * tiles < sms ? units * tiles : sms);
+    const int64_t tiles = ((int64_t)max_past + n_nodes + KV_TILE - 1) / KV_TILE;
+    const int64_t all = (int64_t)n_seqs * n_kv_heads * tiles, groups = sms / t.row_blocks > 1 ? sms / t.row_blocks : 1;
+    t.n_groups = (int)(all < groups ? all : groups);
     t.splits = tiles > 1;
     return t;
 }
 
 cudaError_t tree_attn_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, void* out, float* lse,
-                             float* ws, cudaStream_t s) {
+                             void* ws, cudaStream_t s) {
     uint16_t* o = (uint16_t*)out;
-    if (head_dim == 64) return bf ? launch_all<true, 64>(p, plan, o, lse, ws, s) : launch_all<false, 64>(p, plan, o, lse, ws, s);
-    return bf ? launch_all<true, 128>(p, plan, o, lse, ws, s) : launch_all<false, 128>(p, plan, o, lse, ws, s);
+    int* err = (int*)ws;
+    float* parts = (float*)((uint8_t*)ws + TREE_WS_HEAD);
+    if (head_dim == 64)
+        return bf ? launch_all<true, 64>(p, plan, o, lse, parts, err, s) : launch_all<false, 64>(p, plan, o, lse, parts, err, s);
+    return bf ? launch_all<true, 128>(p, plan, o, lse, parts, err, s) : launch_all<false, 128>(p, plan, o, lse, parts, err, s);
 }
 
 }  // namespace jinf
