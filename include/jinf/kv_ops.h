@@ -59,15 +59,17 @@ jinf_status jinf_b200_tree_mask(const int32_t* parents, int n_nodes, uint32_t* m
 // caller has stored the nodes' own K/V:
 //   out = sum_j softmax_j(scale q.k_j) v_j,  lse = ln sum_j e^(scale q.k_j)
 // q [n_seqs][n_nodes][n_heads][head_dim] in the cache's type, sequences and nodes q_seq_stride
-// and q_node_stride elements apart (multiples of 8, q 16-byte aligned); query head h reads kv
-// head h / (n_heads / n_kv_heads). out is dense in the same order and type; lse (may be NULL)
+// and q_node_stride elements apart (multiples of 8, not 0 unless there is one, q 16-byte aligned);
+// query head h reads kv head h / (n_heads / n_kv_heads), at most JINF_TREE_MAX_GROUP of them each. out is dense in the same order and type; lse (may be NULL)
 // fp32 [n_seqs][n_nodes][n_heads]. mask: device, [n_nodes][ceil(n_nodes / 32)] words, sequence s's
 // at mask + s mask_seq_stride (0: one mask for all); NULL: node t sees nodes 0..t (n_nodes = 1 is
 // plain decode). A row that attends nothing gives out 0 and lse -inf; what masked and unused
 // cache rows hold, NaN included, does not matter.
 // n_past: device int32 [n_seqs], each clamped to 0..max_past; max_past + n_nodes <= max_ctx.
-// scale > 0. workspace: tree_attention_workspace_bytes for the same arguments, zeroed once before
-// first use, then reusable on the same stream; calls that overlap in time need one each.
+// scale > 0. workspace (16-byte aligned): tree_attention_workspace_bytes for the same arguments,
+// zeroed once before first use, then reusable on the same stream; calls that overlap in time need
+// one each. Its first int32 becomes 1 if a wait inside the kernel ran out (the output is then
+// incomplete, and the workspace is to be zeroed again).
 size_t jinf_b200_tree_attention_workspace_bytes(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past);
 jinf_status jinf_b200_tree_attention(void* out, float* lse, const void* q, int64_t q_seq_stride,
                                      int64_t q_node_stride, int n_heads, int n_nodes, const jinf_b200_kv* kv,

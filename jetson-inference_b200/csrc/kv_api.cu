@@ -35,11 +35,13 @@ static bool kv_ok(const jinf_b200_kv* kv) {
 static bool tree_shape_ok(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past) {
     return kv_ok(kv) && n_heads >= 1 && n_heads % kv->n_kv_heads == 0 && n_nodes >= 1 &&
            n_nodes <= JINF_TREE_MAX_NODES && max_past >= 0 && max_past <= kv->max_ctx - n_nodes &&
-           n_heads / kv->n_kv_heads <= JINF_TREE_MAX_GROUP;
+           n_heads / kv->n_kv_heads <= JINF_TREE_MAX_GROUP &&
+           // the kernels number the key tiles of all sequences and heads in 32 bits
+           (int64_t)kv->n_seqs * kv->n_kv_heads * (((int64_t)max_past + n_nodes + KV_TILE - 1) / KV_TILE) <= INT32_MAX;
 }
 
 static TreePlan plan_of(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past) {
-    return tree_plan(kv->n_seqs, kv->n_kv_heads, n_nodes * (n_heads / kv->n_kv_heads), n_nodes, max_past, kv_device_sms(),
+    return tree_plan(kv->n_seqs, kv->n_kv_heads, n_heads / kv->n_kv_heads, n_nodes, max_past, kv_device_sms(),
                      tree_mma_fits(kv));
 }
 
@@ -66,13 +68,18 @@ static void tree_params(TreeParams* p, const void* q, int64_t q_seq, int64_t q_n
     p->max_past = max_past;
     p->max_ctx = kv->max_ctx;
     p->n_rows = n_nodes * p->group;
+    p->tile_nodes = 128 / p->group;
     p->row_blocks = 1;
     p->block_rows = p->n_rows;
     p->scale = scale;
 }
 
-static bool query_ok(const void* q, int64_t q_seq, int64_t q_node, float scale) {
-    return q && aligned16(q) && q_seq % 8 == 0 && q_node % 8 == 0 && isfinite(scale) && scale > 0.f;
+// strides below 2^40 bytes and not 0 where they are used (queries are copied by tensor maps)
+static bool query_ok(const jinf_b200_kv* kv, int n_nodes, const void* q, int64_t q_seq, int64_t q_node, float scale) {
+    auto ok = [](int n, int64_t stride) {
+        return stride % 8 == 0 && (n == 1 || (stride > 0 && stride < ((int64_t)1 << 39)));
+    };
+    return q && aligned16(q) && ok(kv->n_seqs, q_seq) && ok(n_nodes, q_node) && isfinite(scale) && scale > 0.f;
 }
 
 extern "C" jinf_status jinf_b200_tree_mask(const int32_t* parents, int n_nodes, uint32_t* mask) {
@@ -99,7 +106,7 @@ extern "C" jinf_status jinf_b200_tree_attention(void* out, float* lse, const voi
                                                 const uint32_t* mask, int64_t mask_seq_stride, float scale,
                                                 void* workspace, cudaStream_t stream) {
     if (!out || !aligned16(out) || !n_past || !workspace || !aligned16(workspace) || mask_seq_stride < 0 ||
-        !tree_shape_ok(kv, n_heads, n_nodes, max_past) || !query_ok(q, q_seq_stride, q_node_stride, scale))
+        !tree_shape_ok(kv, n_heads, n_nodes, max_past) || !query_ok(kv, n_nodes, q, q_seq_stride, q_node_stride, scale))
         return JINF_ERR_INVALID;
     TreeParams p;
     tree_params(&p, q, q_seq_stride, q_node_stride, n_heads, n_nodes, kv, n_past, max_past, mask, mask_seq_stride, scale);
@@ -118,7 +125,7 @@ extern "C" jinf_status jinf_b200_attention_mass(float* mass, const void* q, int6
                                                 const float* lse, const uint32_t* mask, int64_t mask_seq_stride,
                                                 const float* node_weight, float scale, cudaStream_t stream) {
     if (!mass || !n_past || !lse || mask_seq_stride < 0 || !tree_shape_ok(kv, n_heads, n_nodes, max_past) ||
-        !query_ok(q, q_seq_stride, q_node_stride, scale))
+        !query_ok(kv, n_nodes, q, q_seq_stride, q_node_stride, scale))
         return JINF_ERR_INVALID;
     TreeParams p;
     tree_params(&p, q, q_seq_stride, q_node_stride, n_heads, n_nodes, kv, n_past, max_past, mask, mask_seq_stride, scale);

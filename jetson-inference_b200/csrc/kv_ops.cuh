@@ -27,6 +27,7 @@ struct TreeParams {
     int n_rows;      // query rows of a kv head: n_nodes * group, row r = node r / group, head r % group
     int row_blocks;  // blocks of query rows a kv head's rows are divided into
     int block_rows;  // rows of a block (the last may have fewer)
+    int tile_nodes;  // k_tree_mma: nodes whose rows fill one tile of 128 query rows
     float scale;
 };
 
@@ -96,24 +97,30 @@ constexpr int KV_TILE = 128;
 __device__ __forceinline__ int seq_tiles(const TreeParams& p, int past) {
     return (past + p.n_nodes + KV_TILE - 1) / KV_TILE;
 }
-// Groups that get a share: none is empty, so the parts of a unit are those of consecutive groups.
-__device__ __forceinline__ int share_count(int64_t total, int n) { return (int)min((int64_t)n, total); }
-__device__ __forceinline__ int64_t share_start(int64_t total, int g, int n) { return total * g / n; }
-// The group whose share holds tile t.
-__device__ __forceinline__ int share_owner(int64_t total, int64_t t, int n) {
-    int g = (int)((t * n) / total);
-    while (g + 1 < n && share_start(total, g + 1, n) <= t) ++g;
-    while (g > 0 && share_start(total, g, n) > t) --g;
-    return g;
-}
+// Shares of n groups (at most as many as tiles, so that none is empty and the parts of a unit are
+// those of consecutive groups): the first `more` take each + 1 tiles, the others `each`. The host
+// refuses shapes of 2^31 tiles and more.
+struct Shares {
+    int n, each, more;
+    Shares() = default;
+    __device__ __forceinline__ Shares(int total, int groups) : n(min(groups, total)), each(total / n), more(total - each * n) {}
+    __device__ __forceinline__ int start(int g) const { return g * each + min(g, more); }
+    __device__ __forceinline__ int owner(int t) const {  // of tile t
+        return t < more * (each + 1) ? t / (each + 1) : more + (t - more * (each + 1)) / each;
+    }
+};
 
 // A part of a unit: tiles t0..t1 - 1 of its `tiles`.
 struct Segment {
     int seq, head, past, tiles, t0, t1;
 };
+// A unit that several groups share: which, and the groups of its first and last part.
+struct SharedUnit {
+    int seq, head, g0, g1;
+};
 // A group's share, walked segment by segment.
 struct Share {
-    int64_t left;  // tiles not yet handed out
+    int left;  // tiles not yet handed out
     int seq, head, tile;
 
     __device__ __forceinline__ bool next(const TreeParams& p, Segment& s) {
@@ -123,7 +130,7 @@ struct Share {
         s.past = clamped_past(p, seq);
         s.tiles = seq_tiles(p, s.past);
         s.t0 = tile;
-        s.t1 = (int)min((int64_t)s.tiles, tile + left);
+        s.t1 = min(s.tiles, tile + left);
         left -= s.t1 - s.t0;
         tile = 0;
         if (++head == p.n_kv_heads) {
@@ -133,42 +140,71 @@ struct Share {
         return true;
     }
 };
-// Group g's share of n groups, found by one warp (all its lanes get it).
-__device__ __forceinline__ Share share_begin(const TreeParams& p, int g, int n) {
+struct Place {  // of a tile: its sequence, kv head, place in the unit, and the unit's tiles
+    int seq, head, tile, tiles;
+};
+// One warp finds tile t of all (every lane gets it).
+__device__ __forceinline__ Place find_tile(const TreeParams& p, int t) {
     const int lane = threadIdx.x & 31;
-    int64_t sum = 0;
-    for (int s = lane; s < p.n_seqs; s += 32) sum += seq_tiles(p, clamped_past(p, s));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(JINF_FULL_MASK, sum, o);
-    const int64_t total = sum * p.n_kv_heads;
-    n = share_count(total, n);
-    Share sh{0, 0, 0, 0};
-    if (g >= n) return sh;
-    const int64_t begin = share_start(total, g, n);
-    sh.left = share_start(total, g + 1, n) - begin;
-    int64_t base = 0;  // tiles of one head over the sequences before this round's
+    Place at{0, 0, 0, 1};
+    int base = 0;  // tiles of one head over the sequences before this round's
     for (int s0 = 0; s0 < p.n_seqs; s0 += 32) {
-        const int s = s0 + lane, t = s < p.n_seqs ? seq_tiles(p, clamped_past(p, s)) : 0;
-        int64_t upto = t;
+        const int s = s0 + lane, tiles = s < p.n_seqs ? seq_tiles(p, clamped_past(p, s)) : 0;
+        int upto = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(JINF_FULL_MASK, upto, o);
+            const int x = __shfl_up_sync(JINF_FULL_MASK, upto, o);
             if (lane >= o) upto += x;
         }
         upto += base;
-        const uint32_t has = __ballot_sync(JINF_FULL_MASK, upto * p.n_kv_heads > begin);
+        const uint32_t has = __ballot_sync(JINF_FULL_MASK, upto * p.n_kv_heads > t);
         if (has) {
-            const int at = __ffs(has) - 1;
-            const int tiles = __shfl_sync(JINF_FULL_MASK, t, at);
-            const int64_t in_seq = begin - (__shfl_sync(JINF_FULL_MASK, upto, at) - tiles) * p.n_kv_heads;
-            sh.seq = s0 + at;
-            sh.head = (int)(in_seq / tiles);
-            sh.tile = (int)(in_seq % tiles);
-            return sh;
+            const int k = __ffs(has) - 1;
+            at.tiles = __shfl_sync(JINF_FULL_MASK, tiles, k);
+            const int in_seq = t - (__shfl_sync(JINF_FULL_MASK, upto, k) - at.tiles) * p.n_kv_heads;
+            at.seq = s0 + k;
+            at.head = in_seq / at.tiles;
+            at.tile = in_seq - at.head * at.tiles;
+            return at;
         }
         base = __shfl_sync(JINF_FULL_MASK, upto, 31);
     }
+    return at;
+}
+// Group g's share of `groups`, found by one warp (all its lanes get it), and how the tiles are dealt.
+__device__ __forceinline__ Share share_begin(const TreeParams& p, int g, int groups, Shares& all) {
+    int sum = 0;
+    for (int s = threadIdx.x & 31; s < p.n_seqs; s += 32) sum += seq_tiles(p, clamped_past(p, s));
+    sum = (int)__reduce_add_sync(JINF_FULL_MASK, (unsigned)sum);
+    all = Shares(sum * p.n_kv_heads, groups);
+    Share sh{0, 0, 0, 0};
+    if (g >= all.n) return sh;
+    const int begin = all.start(g);
+    const Place at = find_tile(p, begin);
+    sh.left = all.start(g + 1) - begin;
+    sh.seq = at.seq;
+    sh.head = at.head;
+    sh.tile = at.tile;
     return sh;
+}
+// The units that group g shares with others, its first and its last at most; found by one warp.
+__device__ __forceinline__ int shared_units(const TreeParams& p, int g, const Shares& all, SharedUnit (&u)[2]) {
+    if (g >= all.n) return 0;
+    int n = 0;
+    const int begin = all.start(g), end = all.start(g + 1);
+    for (int x = 0; x < 2; ++x) {
+        const int t = x ? end - 1 : begin;
+        const Place at = find_tile(p, t);
+        const int first = t - at.tile, last = first + at.tiles - 1;
+        if (first >= begin && last < end) continue;            // whole
+        if (x && n && u[0].seq == at.seq && u[0].head == at.head) break;  // the same unit
+        u[n].seq = at.seq;
+        u[n].head = at.head;
+        u[n].g0 = all.owner(first);
+        u[n].g1 = all.owner(last);
+        ++n;
+    }
+    return n;
 }
 
 int kv_device_sms();  // SMs of the current device (cached per device)
@@ -177,12 +213,10 @@ int kv_device_sms();  // SMs of the current device (cached per device)
 
 struct TreePlan {
     int row_blocks, block_rows;
-    int n_groups;  // grid: n_groups * row_blocks CTAs
+    int n_groups;  // grid: n_groups * row_blocks CTAs, all resident (one per SM)
     bool mma;      // k_tree_mma, else k_tree_rows
-    bool splits;   // some unit may be shared by several groups
 };
-TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int sms,
-                   bool mma_fits);
+TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_past, int sms, bool mma_fits);
 size_t tree_workspace_bytes(const TreePlan& plan, int head_dim);
 // k_tree_mma's tensor maps describe this cache (their strides are below 2^40 bytes and not 0)
 bool tree_mma_fits(const jinf_b200_kv* kv);

@@ -9,8 +9,8 @@
 // k_tree_rows: up to 32 rows of a kv head at a time. A warp streams its own 16-key chunks (K and
 // V, 16-byte asynchronous copies, a private ring, no CTA barrier), s = Q K^T and O += P V as
 // m16n8k16 fragments with the probabilities staying in registers. Units are dealt to the CTAs
-// by tile (kv_ops.cuh); a CTA's eight warps join their (m, l, O) in shared memory, and
-// k_tree_merge joins what several CTAs hold of one unit.
+// by tile (kv_ops.cuh); a CTA's eight warps join their (m, l, O) in shared memory, and the CTAs
+// of one unit join theirs at the end (tree_part.cuh). More rows go to k_tree_mma (tree_mma.cu).
 #include "kv_ops.cuh"
 #include "tree_part.cuh"
 
@@ -35,7 +35,7 @@ struct RowsSmem {
 
 template <bool BF, int HD, int MT>
 __global__ void __launch_bounds__(TW * 32, 1)
-    k_tree_rows(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, float* __restrict__ parts) {
+    k_tree_rows(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, void* __restrict__ workspace) {
     using SM = RowsSmem<HD, MT>;
     constexpr int CH = HD / 8;       // 16-byte chunks of a row
     constexpr int ROWB = HD * 2;     // bytes of a row
@@ -46,17 +46,24 @@ __global__ void __launch_bounds__(TW * 32, 1)
     float* join = reinterpret_cast<float*>(sm);
     uint8_t* sq = sm + SM::UNION;
     __shared__ Share s_share;
+    __shared__ Shares s_all;
+    __shared__ JoinPlan s_join;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = smem_u32(sm) + warp * (TS * 2 * WKEYS * ROWB);
 
     const int block = blockIdx.x % p.row_blocks, group = blockIdx.x / p.row_blocks;
     const int row0 = block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
     if (warp == 0) {
-        const Share sh = share_begin(p, group, gridDim.x / p.row_blocks);
-        if (lane == 0) s_share = sh;
+        Shares all;
+        const Share sh = share_begin(p, group, gridDim.x / p.row_blocks, all);
+        if (lane == 0) {
+            s_share = sh;
+            s_all = all;
+        }
     }
     __syncthreads();
     Share share = s_share;
+    const TreeWs ws = tree_ws(workspace, gridDim.x);
     const float c2 = p.scale * LOG2E;
 
     for (Segment u; share.next(p, u);) {
@@ -269,7 +276,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
             }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == u.tiles;
-        float* part = parts + ((size_t)blockIdx.x * 2 + (t0 == 0 ? 1 : 0)) * part_floats(p.block_rows, HD);
+        float* part = ws.parts + ((size_t)blockIdx.x * 2 + (t0 == 0 ? 1 : 0)) * part_floats(p.block_rows, HD);
         for (int i = tid; i < rows * (HD / 4); i += TW * 32) {
             const int r = i % rows, d = (i / rows) * 4;
             float M = -INFINITY;
@@ -291,9 +298,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
             if (whole) {
                 const int rr = row0 + r;
                 const size_t orow = ((size_t)u.seq * p.n_nodes + rr / p.group) * p.n_heads + u.head * p.group + rr % p.group;
-                const float inv = L > 0.f ? 1.f / L : L == 0.f ? 1.f : L;  // an empty row stays 0, NaN stays NaN
-                const uint2 w2 = make_uint2(pack2<BF>(a.x * inv, a.y * inv), pack2<BF>(a.z * inv, a.w * inv));
-                *reinterpret_cast<uint2*>(out + orow * HD + d) = w2;
+                store4<BF>(out + orow * HD + d, a, row_inv(L));
                 if (lse && d == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
             } else {
                 *reinterpret_cast<float4*>(part + ((size_t)(d / 4) * p.block_rows + r) * 4) = a;
@@ -305,155 +310,59 @@ __global__ void __launch_bounds__(TW * 32, 1)
         }
         __syncthreads();  // the join area is the ring of the next unit
     }
-    pdl_trigger();
-}
-
-constexpr int MERGE_THREADS = 256;
-
-// Joins the parts of the units that several groups share. blockIdx.x: (sequence, kv head, row
-// block); a thread owns four columns of one row and adds the parts in the groups' order, each
-// scaled by e^(m_part - m), eight parts' loads in flight.
-template <bool BF, int HD>
-__global__ void __launch_bounds__(MERGE_THREADS)
-    k_tree_merge(const TreeParams p, uint16_t* __restrict__ out, float* __restrict__ lse, const float* __restrict__ parts,
-                 int n_groups) {
-    __shared__ int64_t s_before, s_all;  // tiles of one kv head: of the sequences before this one, and of all
-    const int block = blockIdx.x % p.row_blocks, sh = blockIdx.x / p.row_blocks;
-    const int head = sh % p.n_kv_heads, seq = sh / p.n_kv_heads;
-    if (threadIdx.x < 32) {
-        int64_t before = 0, all = 0;
-        for (int s = threadIdx.x; s < p.n_seqs; s += 32) {
-            const int t = seq_tiles(p, clamped_past(p, s));
-            all += t;
-            if (s < seq) before += t;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            before += __shfl_xor_sync(JINF_FULL_MASK, before, o);
-            all += __shfl_xor_sync(JINF_FULL_MASK, all, o);
-        }
-        if (threadIdx.x == 0) {
-            s_before = before;
-            s_all = all;
+    if (warp == 0) {
+        SharedUnit u[2];
+        const int n = shared_units(p, group, s_all, u);
+        if (lane == 0) {
+            s_join.n = n;
+            s_join.unit[0] = u[0];
+            s_join.unit[1] = u[1];
         }
     }
-    __syncthreads();
-    const int64_t total = s_all * p.n_kv_heads;
-    n_groups = share_count(total, n_groups);
-    const int tiles = seq_tiles(p, clamped_past(p, seq));
-    const int64_t first = s_before * p.n_kv_heads + (int64_t)head * tiles;
-    const int g0 = share_owner(total, first, n_groups), g1 = share_owner(total, first + tiles - 1, n_groups);
-    const int row0 = block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
-    const int i = blockIdx.y * MERGE_THREADS + threadIdx.x;
-    pdl_wait();  // the parts below are the previous kernel's
-    if (g0 == g1 || i >= rows * (HD / 4)) return;
-    const int r = i % rows, d4 = i / rows;
-    const size_t pf = part_floats(p.block_rows, HD);
-    const float c2 = p.scale * LOG2E;
-    float M = -INFINITY, L = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int B = 8;
-    for (int gb = g0; gb <= g1; gb += B) {
-        float pm[B], pl[B];
-        float4 po[B];
-#pragma unroll
-        for (int k = 0; k < B; ++k) {
-            const int g = gb + k;
-            pm[k] = -INFINITY;
-            pl[k] = 0.f;
-            po[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (g <= g1) {
-                // the group that begins the unit kept it in its second slot, the others in their first
-                const float* part = parts + (((size_t)g * p.row_blocks + block) * 2 + (g == g0 ? 1 : 0)) * pf;
-                pm[k] = __ldcg(part + (size_t)p.block_rows * HD + r);
-                pl[k] = __ldcg(part + (size_t)p.block_rows * (HD + 1) + r);
-                po[k] = __ldcg(reinterpret_cast<const float4*>(part) + (size_t)d4 * p.block_rows + r);
-            }
-        }
-        float mn = M;
-#pragma unroll
-        for (int k = 0; k < B; ++k) mn = fmaxf(mn, pm[k]);
-        const float base = mn == -INFINITY ? 0.f : mn;
-        const float corr = exp2f((M - base) * c2);
-        M = mn;
-        L *= corr;
-        a.x *= corr; a.y *= corr; a.z *= corr; a.w *= corr;
-#pragma unroll
-        for (int k = 0; k < B; ++k) {
-            const float f = exp2f((pm[k] - base) * c2);
-            L = fmaf(pl[k], f, L);
-            a.x = fmaf(po[k].x, f, a.x);
-            a.y = fmaf(po[k].y, f, a.y);
-            a.z = fmaf(po[k].z, f, a.z);
-            a.w = fmaf(po[k].w, f, a.w);
-        }
-    }
-    const int rr = row0 + r;
-    const size_t orow = ((size_t)seq * p.n_nodes + rr / p.group) * p.n_heads + head * p.group + rr % p.group;
-    const float inv = L > 0.f ? 1.f / L : L == 0.f ? 1.f : L;
-    *reinterpret_cast<uint2*>(out + orow * HD + d4 * 4) =
-        make_uint2(pack2<BF>(a.x * inv, a.y * inv), pack2<BF>(a.z * inv, a.w * inv));
-    if (lse && d4 == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
-}
-
-template <bool BF, int HD, int MT>
-cudaError_t launch_rows(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* parts, cudaStream_t s) {
-    constexpr int smem = RowsSmem<HD, MT>::TOTAL;
-    const cudaError_t e = cudaFuncSetAttribute(k_tree_rows<BF, HD, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    k_tree_rows<BF, HD, MT><<<plan.n_groups * plan.row_blocks, TW * 32, smem, s>>>(p, out, lse, parts);
-    return cudaGetLastError();
+    join_units<BF, HD, TW * 32>(p, s_join, group, block, out, lse, ws);
 }
 
 template <bool BF, int HD>
-cudaError_t launch_all(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* parts, int* err,
-                       cudaStream_t s) {
-    const cudaError_t e = plan.mma                 ? tree_mma_launch(p, plan, BF, HD, out, lse, parts, err, s)
-                          : plan.block_rows <= 16 ? launch_rows<BF, HD, 1>(p, plan, out, lse, parts, s)
-                                                  : launch_rows<BF, HD, 2>(p, plan, out, lse, parts, s);
-    if (e != cudaSuccess || !plan.splits) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.n_seqs * p.n_kv_heads * p.row_blocks),
-                       (unsigned)((p.block_rows * (HD / 4) + MERGE_THREADS - 1) / MERGE_THREADS));
-    cfg.blockDim = dim3(MERGE_THREADS);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_tree_merge<BF, HD>, p, out, lse, (const float*)parts, plan.n_groups);
+cudaError_t launch_rows(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, void* ws, cudaStream_t s) {
+    const int grid = plan.n_groups * plan.row_blocks;
+    return plan.block_rows <= 16
+               ? launch_coop(k_tree_rows<BF, HD, 1>, grid, TW * 32, RowsSmem<HD, 1>::TOTAL, s, p, out, lse, ws)
+               : launch_coop(k_tree_rows<BF, HD, 2>, grid, TW * 32, RowsSmem<HD, 2>::TOTAL, s, p, out, lse, ws);
 }
 
 }  // namespace
 
 size_t tree_workspace_bytes(const TreePlan& plan, int head_dim) {
-    return TREE_WS_HEAD + sizeof(float) * (size_t)plan.n_groups * plan.row_blocks * 2 * part_floats(plan.block_rows, head_dim);
+    const int ctas = plan.n_groups * plan.row_blocks;
+    return tree_ws_head(ctas) + sizeof(float) * (size_t)ctas * 2 * part_floats(plan.block_rows, head_dim);
 }
 
-TreePlan tree_plan(int n_seqs, int n_kv_heads, int n_rows, int n_nodes, int max_past, int sms,
-                   bool mma_fits) {
+TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_past, int sms, bool mma_fits) {
     TreePlan t;
+    const int n_rows = group * n_nodes;
     t.mma = n_rows > 16 && mma_fits;
-    const int most = t.mma ? 256 : 32;
-    t.row_blocks = (n_rows + most - 1) / most;
-    t.block_rows = (n_rows + t.row_blocks - 1) / t.row_blocks;
+    if (t.mma) {  // whole nodes: two tiles of 128 rows hold 2 * (128 / group) of them
+        const int most = 2 * (128 / group), blocks = (n_nodes + most - 1) / most;
+        const int nodes = (n_nodes + blocks - 1) / blocks;
+        t.block_rows = nodes * group;
+    } else {
+        const int blocks = (n_rows + 31) / 32;
+        t.block_rows = (n_rows + blocks - 1) / blocks;
+    }
     t.row_blocks = (n_rows + t.block_rows - 1) / t.block_rows;
     const int64_t tiles = ((int64_t)max_past + n_nodes + KV_TILE - 1) / KV_TILE;
-    const int64_t all = (int64_t)n_seqs * n_kv_heads * tiles, groups = sms / t.row_blocks > 1 ? sms / t.row_blocks : 1;
+    const int64_t all = (int64_t)n_seqs * n_kv_heads * tiles, groups = sms / t.row_blocks;
     t.n_groups = (int)(all < groups ? all : groups);
-    t.splits = tiles > 1;
     return t;
 }
 
 cudaError_t tree_attn_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, void* out, float* lse,
                              void* ws, cudaStream_t s) {
     uint16_t* o = (uint16_t*)out;
-    int* err = (int*)ws;
-    float* parts = (float*)((uint8_t*)ws + TREE_WS_HEAD);
-    if (head_dim == 64)
-        return bf ? launch_all<true, 64>(p, plan, o, lse, parts, err, s) : launch_all<false, 64>(p, plan, o, lse, parts, err, s);
-    return bf ? launch_all<true, 128>(p, plan, o, lse, parts, err, s) : launch_all<false, 128>(p, plan, o, lse, parts, err, s);
+    if (plan.n_groups < 1) return cudaErrorInvalidValue;  // fewer SMs than row blocks
+    if (plan.mma) return tree_mma_launch(p, plan, bf, head_dim, o, lse, ws, s);
+    if (head_dim == 64) return bf ? launch_rows<true, 64>(p, plan, o, lse, ws, s) : launch_rows<false, 64>(p, plan, o, lse, ws, s);
+    return bf ? launch_rows<true, 128>(p, plan, o, lse, ws, s) : launch_rows<false, 128>(p, plan, o, lse, ws, s);
 }
 
 }  // namespace jinf

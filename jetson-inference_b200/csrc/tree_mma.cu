@@ -4,9 +4,10 @@
 // A CTA takes a block of up to 256 query rows (nodes x query heads of a kv head) over its share
 // of key tiles (kv_ops.cuh), 128 keys a tile:
 //   warp 0      copies K and V tiles (TMA boxes of 64 columns x 128 rows, 128B swizzle) into a ring;
-//   warp 1      allocates tensor memory and issues the MMAs: S_w = Q_w K^T (both operands in shared
-//               memory) and O_w += P_w V (P_w in tensor memory over S_w, V MN-major);
-//   warps 2, 3  clean the V tiles that hold rows of the tree or reach past the last key: values
+//   warps 1, 3  issue the MMAs of softmax group w = 0 and 1: S_w = Q_w K^T (both operands in shared
+//               memory) and O_w += P_w V (P_w in tensor memory over S_w, V MN-major). Two warps,
+//               because one issuer's turn for both groups was the longest chain of a tile;
+//   warp 2      cleans the V tiles that hold rows of the tree or reach past the last key: values
 //               behind the end, and values that are not finite (a masked key's V would enter O as
 //               0 * v), become 0, and the keys of the latter are noted;
 //   warps 4-7, 8-11  two softmax groups, one thread per query row: read S_w, keep the running maximum
@@ -40,17 +41,19 @@ struct MmaSmem {
     static constexpr int OFF_KV = 2 * TILE;
     static constexpr int OFF_MISC = OFF_KV + ST * TILE;
     struct Misc {
-        uint64_t full[ST], empty[ST], vok[ST];
-        uint64_t s_full[2], p_ready[2], pv_done[2], q_ready[2], flag_ok[2], join, drain;
+        uint64_t full[ST], empty[ST], vok[BAD_SETS];
+        uint64_t s_full[2][2], p_ready[2][2], pv_done[2], flag_ok[2], drain[2], join, q_full, q_free;
         Share share;
+        Shares all;
+        JoinPlan plan;
         uint32_t tmem;
         int abort;
-        uint32_t bad[BAD_SETS][2][4];  // one part per cleaning warp
+        uint32_t bad[BAD_SETS][4];
         float jm[128], jl[128];
     };
     static constexpr int TOTAL = OFF_MISC + (int)sizeof(Misc) + 1024;
 };
-static_assert(MmaSmem<128>::TOTAL <= 232448 && MmaSmem<64>::TOTAL <= 232448, "shared memory");
+static_assert(MmaSmem<128>::TOTAL + 256 <= 232448 && MmaSmem<64>::TOTAL + 256 <= 232448, "shared memory (with join_units')");
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -76,11 +79,12 @@ __device__ __forceinline__ uint32_t seen_keys(const TreeParams& p, const uint32_
 
 template <bool BF, int HD>
 __global__ void __launch_bounds__(XT, 1)
-    k_tree_mma(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const TreeParams p,
-               uint16_t* __restrict__ out, float* __restrict__ lse, float* __restrict__ parts, int* __restrict__ err) {
+    k_tree_mma(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+               const __grid_constant__ CUtensorMap tmv, const TreeParams p, uint16_t* __restrict__ out,
+               float* __restrict__ lse, void* __restrict__ workspace) {
     using SM = MmaSmem<HD>;
     constexpr int TILE = SM::TILE, ST = SM::ST;
-    constexpr uint32_t ID_QK = umma_idesc(BF, 128, 128, false), ID_PV = umma_idesc(BF, 128, HD, true);
+    constexpr uint32_t ID_QK = umma_idesc(BF, 128, 64, false), ID_PV = umma_idesc(BF, 128, HD, true);
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     typename SM::Misc& ms = *reinterpret_cast<typename SM::Misc*>(sm + SM::OFF_MISC);
@@ -88,23 +92,28 @@ __global__ void __launch_bounds__(XT, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int block = blockIdx.x % p.row_blocks, group = blockIdx.x / p.row_blocks;
     const int row0 = block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
-    const bool two = rows > 128;  // two row tiles, one per softmax group; else alternate key tiles
+    const int tile_rows = p.tile_nodes * p.group;
+    const bool two = rows > tile_rows;  // two row tiles, one per softmax group; else alternate key tiles
+    const TreeWs ws = tree_ws(workspace, gridDim.x);
 
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
             mb_init(su32(&ms.full[i]), 1);
-            mb_init(su32(&ms.empty[i]), 1);
-            mb_init(su32(&ms.vok[i]), 64);
+            mb_init(su32(&ms.empty[i]), two ? 2 : 1);  // a tile is used by both groups, or by one
         }
+        for (int i = 0; i < BAD_SETS; ++i) mb_init(su32(&ms.vok[i]), 1);
         for (int w = 0; w < 2; ++w) {
-            mb_init(su32(&ms.s_full[w]), 1);
-            mb_init(su32(&ms.p_ready[w]), 128);
+            for (int h = 0; h < 2; ++h) {
+                mb_init(su32(&ms.s_full[w][h]), 1);
+                mb_init(su32(&ms.p_ready[w][h]), 4);
+            }
             mb_init(su32(&ms.pv_done[w]), 1);
-            mb_init(su32(&ms.q_ready[w]), 128);
             mb_init(su32(&ms.flag_ok[w]), 1);
+            mb_init(su32(&ms.drain[w]), 1);
         }
-        mb_init(su32(&ms.join), 256);
-        mb_init(su32(&ms.drain), 1);
+        mb_init(su32(&ms.join), 8);
+        mb_init(su32(&ms.q_full), 1);
+        mb_init(su32(&ms.q_free), 6);  // both issuers, and group 0's warps, which join over Q's memory
         ms.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -113,8 +122,12 @@ __global__ void __launch_bounds__(XT, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (warp == 2) {
-        const Share sh = share_begin(p, group, gridDim.x / p.row_blocks);
-        if (lane == 0) ms.share = sh;
+        Shares all;
+        const Share sh = share_begin(p, group, gridDim.x / p.row_blocks, all);
+        if (lane == 0) {
+            ms.share = sh;
+            ms.all = all;
+        }
     }
     tc_before_sync();
     __syncthreads();
@@ -131,12 +144,18 @@ __global__ void __launch_bounds__(XT, 1)
             if ((it & 255) == 255 && *(volatile int*)&ms.abort) return false;
         }
         atomicExch(&ms.abort, 1);
-        atomicExch(err, 1);
+        atomicExch(ws.err, 1);
         return false;
     };
     // the same for a whole warp, which stays converged
     auto wait_all = [&](uint64_t& bar, uint32_t parity) -> bool {
         return __all_sync(JINF_FULL_MASK, wait(bar, parity));
+    };
+    // One arrival per warp, after what all its lanes did: 128 of them on one mbarrier would take about
+    // 1200 cycles.
+    auto arrive_warp = [&](uint64_t& bar) {
+        __syncwarp();
+        if (lane == 0) mb_arrive(su32(&bar));
     };
     // Ring positions of a segment of n tiles, from its base: K_0, then K_(i+1), V_i for every i (the
     // order in which the MMAs take them), the last V_i without a K.
@@ -145,10 +164,20 @@ __global__ void __launch_bounds__(XT, 1)
 
     if (warp == 0) {
         if (lane == 0) {  // ---- copies
-            uint32_t pos = 0;
+            uint32_t pos = 0, units = 0;
             bool ok = true;
             while (ok && share.next(p, sg)) {
                 const int n = sg.t1 - sg.t0;
+                // Q: the rows of tile_nodes nodes, node by node, are one box; nodes past the last are zeros
+                if (units && !(ok = wait(ms.q_free, (units - 1) & 1))) break;
+                const uint32_t qbar = su32(&ms.q_full);
+                mb_expect(qbar, (two ? 2 : 1) * (HD / 64) * 128 * tile_rows);
+                for (int w = 0; w < (two ? 2 : 1); ++w)
+#pragma unroll
+                    for (int a = 0; a < HD / 64; ++a)
+                        tma_load_4d(s_q + w * TILE + a * ATOM, &tmq, 64 * a, sg.head * p.group,
+                                    row0 / p.group + w * p.tile_nodes, sg.seq, qbar);
+                ++units;
                 for (int x = 0; ok && x < 2 * n; ++x, ++pos) {
                     // x-th of the order above
                     const bool is_k = x == 0 || ((x & 1) && x < 2 * n - 1);
@@ -163,84 +192,93 @@ __global__ void __launch_bounds__(XT, 1)
                                     sg.head, sg.seq, bar);
                 }
             }
-            if (!ok)  // leave no copy in flight
+            if (!ok) {  // leave no copy in flight
+                if (units) mb_wait(su32(&ms.q_full), (units - 1) & 1);
                 for (uint32_t s = 0; s < ST && s < pos; ++s) mb_wait(su32(&ms.full[s]), ((pos - 1 - s) / ST) & 1);
+            }
         }
-    } else if (warp == 1) {
-        if (lane == 0) {  // ---- MMAs
-            uint32_t base = 0, np[2] = {0, 0}, nq[2] = {0, 0}, vok_ph = 0;
-            bool ok = true;
-            auto full = [&](uint32_t pos) { return wait(ms.full[pos % ST], (pos / ST) & 1); };
-            auto qk = [&](int w, uint32_t pos) {
-                tc_after_sync();
-                const uint32_t a = s_q + w * TILE, b = s_kv + (pos % ST) * TILE;
+    } else if (warp == 1 || warp == 3) {
+        // ---- MMAs of group w, one lane issuing for the converged warp
+        const int w = warp == 3, step = two ? 1 : 2;
+        const bool leader = elect_one();
+        const uint32_t t_s = tmem + 128 * w, t_o = tmem + 256 + 128 * w;
+        const uint64_t dq = umma_desc(s_q + (two ? w : 0) * TILE);
+        uint32_t base = 0, done = 0, units = 0, ord = 0;
+        bool ok = true;
+        auto full = [&](uint32_t pos) { return wait_all(ms.full[pos % ST], (pos / ST) & 1); };
+        auto qk = [&](uint32_t pos, int h) {
+            const uint64_t dk = umma_desc(s_kv + (pos % ST) * TILE + h * 8192);
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * ATOM + (kk & 3) * 32;
-                    umma_ss(tmem + 128 * w, umma_desc(a + off), umma_desc(b + off), ID_QK, kk > 0);
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t off = ((kk >> 2) * ATOM + (kk & 3) * 32) >> 4;
+                umma_ss(t_s + 64 * h, dq + off, dk + off, ID_QK, kk > 0);
+            }
+            umma_commit(su32(&ms.s_full[w][h]));
+        };
+        while (ok && share.next(p, sg)) {
+            const int n = sg.t1 - sg.t0, first_tail = max(0, sg.past / KV_TILE - sg.t0);
+            int i = two ? 0 : w;
+            if (i < n) {
+                const uint32_t k = base + pos_k(i);
+                if (!(ok = wait_all(ms.q_full, units & 1) && full(k))) break;
+                tc_after_sync();
+                if (leader) {
+                    qk(k, 0);
+                    qk(k, 1);
+                    umma_commit(su32(&ms.empty[k % ST]));
                 }
-                umma_commit(su32(&ms.s_full[w]));
-            };
-            auto pv = [&](int w, uint32_t pos, bool accumulate) {
-                tc_after_sync();
-                const uint32_t b = s_kv + (pos % ST) * TILE;
+                __syncwarp();
+            }
+            for (; i < n; i += step) {
+                const uint32_t v = base + pos_v(i, n), k = base + pos_k(i + step);
+                const uint64_t dv = umma_desc(s_kv + (v % ST) * TILE, ATOM);
+                const bool tail = i >= first_tail, more = i + step < n;
+                if (tail) {
+                    const uint32_t o = ord + i - first_tail;
+                    if (!(ok = wait_all(ms.vok[o % BAD_SETS], (o / BAD_SETS) & 1))) break;
+                }
+                if (!(ok = full(v))) break;
+                if (more && !(ok = full(k))) break;
 #pragma unroll
-                for (int kk = 0; kk < KV_TILE / 16; ++kk)
-                    umma_ts(tmem + 256 + 128 * w, tmem + 128 * w + 8 * kk, umma_desc(b + kk * 2048, ATOM), ID_PV,
-                            accumulate || kk > 0);
-                umma_commit(su32(&ms.pv_done[w]));
-            };
-            while (ok && share.next(p, sg)) {
-                const int n = sg.t1 - sg.t0;
-                if (!(ok = full(base))) break;
-                for (int w = 0; w < (two ? 2 : 1); ++w) {
-                    if (!(ok = wait(ms.q_ready[w], nq[w]++ & 1))) break;
-                    qk(w, base);
+                for (int h = 0; h < 2; ++h) {
+                    if (!(ok = wait_all(ms.p_ready[w][h], done & 1))) break;
+                    tc_after_sync();
+                    if (leader) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_ts(t_o, t_s + 64 * h + 8 * kk, dv + ((4 * h + kk) * 2048 >> 4), ID_PV, i >= step || h || kk > 0);
+                        umma_commit(su32(&ms.pv_done[w]));
+                        if (h == 1) umma_commit(su32(&ms.empty[v % ST]));
+                        if (more) qk(k, h);
+                        if (more && h == 1) umma_commit(su32(&ms.empty[k % ST]));
+                        if (tail && h == 1) mb_arrive(su32(&ms.flag_ok[w]));
+                    }
+                    __syncwarp();
                 }
                 if (!ok) break;
-                umma_commit(su32(&ms.empty[base % ST]));
-                if (!two && n > 1) {
-                    const uint32_t k1 = base + pos_k(1);
-                    if (!(ok = full(k1) && wait(ms.q_ready[1], nq[1]++ & 1))) break;
-                    qk(1, k1);
-                    umma_commit(su32(&ms.empty[k1 % ST]));
-                }
-                for (int i = 0; ok && i < n; ++i) {
-                    const uint32_t v = base + pos_v(i, n);
-                    const bool tail = (sg.t0 + i + 1) * KV_TILE > sg.past;
-                    if (!(ok = full(v))) break;
-                    if (tail) {
-                        const uint32_t s = v % ST;
-                        if (!(ok = wait(ms.vok[s], (vok_ph >> s) & 1))) break;
-                        vok_ph ^= 1u << s;
-                    }
-                    // the tile whose scores come next in the group's turn
-                    const int step = two ? 1 : 2;
-                    const bool more = i + step < n;
-                    const uint32_t k = base + pos_k(i + step);
-                    for (int x = 0; x < (two ? 2 : 1); ++x) {
-                        const int w = two ? x : i & 1;
-                        if (!(ok = wait(ms.p_ready[w], np[w]++ & 1))) break;
-                        pv(w, v, two ? i > 0 : i > 1);
-                        if (tail) mb_arrive(su32(&ms.flag_ok[w]));
-                        if (more) {
-                            if (x == 0 && !(ok = full(k))) break;
-                            qk(w, k);
-                        }
-                    }
-                    if (!ok) break;
-                    umma_commit(su32(&ms.empty[v % ST]));
-                    if (more) umma_commit(su32(&ms.empty[k % ST]));
-                }
-                base += 2 * n;
+                ++done;
             }
-            if (!ok) {  // the MMAs already issued finish before the memory goes
-                umma_commit(su32(&ms.drain));
-                mb_wait(su32(&ms.drain), 0);
+            if (!ok) break;
+            if (leader) umma_commit(su32(&ms.q_free));
+            ++units;
+            base += 2 * n;
+            ord += n - min(n, first_tail);
+        }
+        if (!ok && leader) {  // the MMAs already issued finish before the memory goes
+            umma_commit(su32(&ms.drain[w]));
+            mb_wait(su32(&ms.drain[w]), 0);
+        }
+    } else if (warp == 2) {
+        // ---- the units to join at the end, then: clean the tail tiles' V
+        {
+            SharedUnit u[2];
+            const int n = shared_units(p, group, ms.all, u);
+            if (lane == 0) {
+                ms.plan.n = n;
+                ms.plan.unit[0] = u[0];
+                ms.plan.unit[1] = u[1];
             }
         }
-    } else if (warp < 4) {
-        // ---- clean the tail tiles' V
         uint32_t base = 0, ord = 0;
         bool ok = true;
         while (ok && share.next(p, sg)) {
@@ -248,43 +286,42 @@ __global__ void __launch_bounds__(XT, 1)
             for (int i = max(0, sg.past / KV_TILE - sg.t0); i < n; ++i, ++ord) {
                 const uint32_t pos = base + pos_v(i, n);
                 if (!(ok = wait_all(ms.full[pos % ST], (pos / ST) & 1))) break;
-                uint32_t* bad = ms.bad[ord % BAD_SETS][warp - 2];
+                uint32_t* bad = ms.bad[ord % BAD_SETS];
                 if (lane < 4) bad[lane] = 0;
                 __syncwarp();
-                uint8_t* v = sm + SM::OFF_KV + (pos % ST) * TILE;
                 const int key0 = (sg.t0 + i) * KV_TILE;
-                for (int x = tid - 64; x < TILE / 16; x += 64) {
-                    const int kk = (x >> 3) & 127, key = key0 + kk;
-                    if (key < sg.past) continue;
-                    uint4* at = reinterpret_cast<uint4*>(v) + x;
-                    uint4 y = *at;
-                    bool change = false;
-                    if (key >= n_keys) {
-                        y = make_uint4(0u, 0u, 0u, 0u);
-                        change = true;
-                    } else {
-                        uint32_t* w = reinterpret_cast<uint32_t*>(&y);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (nonfinite2<BF>(w[e])) {
+                const int lo = max(0, sg.past - key0), hi = min(KV_TILE, n_keys - key0);  // the tree's rows here
+                uint4* v = reinterpret_cast<uint4*>(sm + SM::OFF_KV + (pos % ST) * TILE);
+                for (int a = 0; a < HD / 64; ++a, v += ATOM / 16) {
+                    for (int x = 8 * hi + lane; x < 8 * KV_TILE; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 8
+                    for (int x = 8 * lo + lane; x < 8 * hi; x += 32) {
+                        uint4 y = v[x];
+                        // an exponent of all ones carries into bit 15 of its half
+                        constexpr uint32_t ONE = BF ? 0x00800080u : 0x04000400u;
+                        if ((((y.x & 0x7FFF7FFFu) + ONE) | ((y.y & 0x7FFF7FFFu) + ONE) | ((y.z & 0x7FFF7FFFu) + ONE) |
+                             ((y.w & 0x7FFF7FFFu) + ONE)) & 0x80008000u) {
+                            uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+                            for (int e = 0; e < 4; ++e) {
                                 if (nonfinite2<BF>(w[e] & 0xFFFFu)) w[e] &= 0xFFFF0000u;
                                 if (nonfinite2<BF>(w[e] & 0xFFFF0000u)) w[e] &= 0xFFFFu;
-                                change = true;
                             }
-                        if (change) atomicOr(&bad[kk >> 5], 1u << (kk & 31));
+                            v[x] = y;
+                            atomicOr(&bad[x >> 8], 1u << ((x >> 3) & 31));
+                        }
                     }
-                    if (change) *at = y;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mb_arrive(su32(&ms.vok[pos % ST]));
+                arrive_warp(ms.vok[ord % BAD_SETS]);
             }
             base += 2 * n;
         }
     } else {
         // ---- softmax groups
         const int w = (warp - 4) >> 2, r = tid - 128 - 128 * w;  // row of the group's tile
-        const int br = two ? 128 * w + r : r;                     // row of the block
-        const bool valid = br < rows, warp_on = (two ? 128 * w : 0) + 32 * (warp & 3) < rows;
+        const int first_row = two ? tile_rows * w : 0, br = first_row + r;  // row of the block
+        const int tile_on = min(tile_rows, rows - first_row);               // rows of the group's tile in use
+        const bool valid = r < tile_on, warp_on = 32 * (warp & 3) < tile_on;
         const int rr = valid ? row0 + br : row0, node = rr / p.group, head_in = rr % p.group;
         const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t t_s = tmem + lane_off + 128 * w, t_o = tmem + lane_off + 256 + 128 * w;
@@ -294,7 +331,7 @@ __global__ void __launch_bounds__(XT, 1)
         uint32_t joins = 0;
         bool ok = true;
         auto meet = [&]() {  // both groups
-            mb_arrive(su32(&ms.join));
+            arrive_warp(ms.join);
             return wait_all(ms.join, joins++ & 1);
         };
         while (ok && share.next(p, sg)) {
@@ -303,115 +340,96 @@ __global__ void __launch_bounds__(XT, 1)
             const int first_tail = max(0, sg.past / KV_TILE - sg.t0);  // of the segment
             const bool mine = two || w < n;                            // the group has a tile
             float m = -INFINITY, l = 0.f;
-            if (mine) {
-                if (valid) {
-                    const uint4* src = reinterpret_cast<const uint4*>(
-                        p.q + (sg.seq * p.q_seq + node * p.q_node + (int64_t)(sg.head * p.group + head_in) * HD) * 2);
-                    uint8_t* dst = sm + w * TILE + (r >> 3) * 1024 + (r & 7) * 128;
-#pragma unroll
-                    for (int c = 0; c < HD / 8; ++c)
-                        *reinterpret_cast<uint4*>(dst + (c >> 3) * ATOM + (((c & 7) ^ (r & 7)) << 4)) = __ldg(src + c);
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mb_arrive(su32(&ms.q_ready[w]));
-            }
             for (int i = two ? 0 : w; i < n; i += step) {
                 const bool tail = i >= first_tail;
-                if (!(ok = wait_all(ms.s_full[w], done & 1))) break;
-                tc_after_sync();
-                if (warp_on) {
-                    const int u0 = (sg.t0 + i) * KV_TILE - sg.past;
-                    // two columns blocks of 32 scores at a time; read again below rather than kept, which
-                    // would take 128 registers
-                    auto scores = [&](int c, uint32_t (&a)[32], uint32_t (&b)[32]) {
-                        tmem_ld32(t_s + 32 * c, a);
-                        tmem_ld32(t_s + 32 * c + 32, b);
+                const int u0 = (sg.t0 + i) * KV_TILE - sg.past;
+#pragma unroll 1
+                for (int h = 0; h < 2; ++h) {
+                    if (!(ok = wait_all(ms.s_full[w][h], done & 1))) break;
+                    tc_after_sync();
+                    if (warp_on) {
+                        uint32_t v[2][32];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) tmem_ld32(t_s + 64 * h + 32 * c, v[c]);
                         tmem_wait_ld();
-                        tmem_pin32(a);
-                        tmem_pin32(b);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) tmem_pin32(v[c]);
                         if (tail) {
-                            const uint32_t sa = seen_keys(p, mask, node, u0 + 32 * c);
-                            const uint32_t sb = seen_keys(p, mask, node, u0 + 32 * c + 32);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                if (!((sa >> j) & 1u)) a[j] = 0xFF800000u;
-                                if (!((sb >> j) & 1u)) b[j] = 0xFF800000u;
+                            for (int c = 0; c < 2; ++c) {
+                                const uint32_t see = seen_keys(p, mask, node, u0 + 64 * h + 32 * c);
+#pragma unroll
+                                for (int j = 0; j < 32; ++j)
+                                    if (!((see >> j) & 1u)) v[c][j] = 0xFF800000u;
                             }
                         }
-                    };
-                    uint32_t va[32], vb[32];
-                    float mx = -INFINITY;
+                        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 4; c += 2) {
-                        scores(c, va, vb);
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) mx = fmaxf(mx, fmaxf(__uint_as_float(va[j]), __uint_as_float(vb[j])));
-                    }
-                    if (i < step) {
-                        m = mx;
-                    } else {
-                        const bool need = mx > m + grow;  // also when nothing was seen yet (m = -inf)
-                        if (__any_sync(JINF_FULL_MASK, need)) {
-                            const float f = need ? ex2((m - mx) * c2) : 1.f;
-                            if (need) m = mx;
-                            l *= f;
-                            ok = wait_all(ms.pv_done[w], (done - 1) & 1);
-                            tc_after_sync();
-                            for (int c = 0; c < HD / 32; ++c) {
-                                uint32_t o[32];
-                                tmem_ld32(t_o + 32 * c, o);
-                                tmem_wait_ld();
-                                tmem_pin32(o);
+                            for (int j = 0; j < 32; j += 2)
+                                mx4[2 * c + ((j >> 1) & 1)] =
+                                    fmaxf(mx4[2 * c + ((j >> 1) & 1)], fmaxf(__uint_as_float(v[c][j]), __uint_as_float(v[c][j + 1])));
+                        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                        if (i < step && h == 0) {
+                            m = mx;
+                        } else {
+                            const bool need = mx > m + grow;  // also when nothing was seen yet (m = -inf)
+                            if (__any_sync(JINF_FULL_MASK, need)) {
+                                const float f = need ? ex2((m - mx) * c2) : 1.f;
+                                if (need) m = mx;
+                                l *= f;
+                                ok = wait_all(ms.pv_done[w], (2 * done + h - 1) & 1);
+                                tc_after_sync();
+#pragma unroll 1
+                                for (int c = 0; c < HD / 32; ++c) {
+                                    uint32_t o[32];
+                                    tmem_ld32(t_o + 32 * c, o);
+                                    tmem_wait_ld();
+                                    tmem_pin32(o);
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                                tmem_st32(t_o + 32 * c, o);
+                                    for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                                    tmem_st32(t_o + 32 * c, o);
+                                }
+                                tmem_wait_st();
                             }
-                            tmem_wait_st();
                         }
-                    }
-                    const float mb = m == -INFINITY ? 0.f : m * c2;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int c = 0; c < 4; c += 2) {
-                        scores(c, va, vb);
+                        const float mb = m == -INFINITY ? 0.f : m * c2;
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
                         uint32_t pk[32];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const float a = ex2(fmaf(__uint_as_float(va[2 * j]), c2, -mb));
-                            const float b = ex2(fmaf(__uint_as_float(va[2 * j + 1]), c2, -mb));
-                            const float e = ex2(fmaf(__uint_as_float(vb[2 * j]), c2, -mb));
-                            const float f = ex2(fmaf(__uint_as_float(vb[2 * j + 1]), c2, -mb));
-                            sum[0] += a;
-                            sum[1] += b;
-                            sum[2] += e;
-                            sum[3] += f;
-                            pk[j] = pack2<BF>(a, b);
-                            pk[16 + j] = pack2<BF>(e, f);
-                        }
-                        // over scores of column 32 c / 2 and on, which have been read
-                        tmem_st32(t_s + 16 * c, pk);
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const float a = ex2(fmaf(__uint_as_float(v[c][2 * j]), c2, -mb));
+                                const float b = ex2(fmaf(__uint_as_float(v[c][2 * j + 1]), c2, -mb));
+                                sum[j & 1] += a;
+                                sum[2 + (j & 1)] += b;
+                                pk[16 * c + j] = pack2<BF>(a, b);
+                            }
+                        tmem_st32(t_s + 64 * h, pk);
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        tmem_wait_st();
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_wait_st();
+                    tc_before_sync();
+                    arrive_warp(ms.p_ready[w][h]);
                 }
-                tc_before_sync();
-                mb_arrive(su32(&ms.p_ready[w]));
+                if (!ok) break;
                 ++done;
                 if (tail) {
-                    const uint32_t(*notes)[4] = ms.bad[(ord + i - first_tail) % BAD_SETS];
+                    const uint32_t* notes = ms.bad[(ord + i - first_tail) % BAD_SETS];
                     if (!(ok = wait_all(ms.flag_ok[w], tails++ & 1))) break;
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) any |= notes[0][x] | notes[1][x];
+                    const uint32_t any = notes[0] | notes[1] | notes[2] | notes[3];
                     if (any && warp_on) {  // values that are not finite, to the rows that see their key
-                        ok = wait_all(ms.pv_done[w], (done - 1) & 1);
+                        ok = wait_all(ms.pv_done[w], 1);
                         tc_after_sync();
                         for (int kk = 0; kk < KV_TILE; ++kk) {
-                            if (!(((notes[0][kk >> 5] | notes[1][kk >> 5]) >> (kk & 31)) & 1u)) continue;
+                            if (!((notes[kk >> 5] >> (kk & 31)) & 1u)) continue;
                             const int key = (sg.t0 + i) * KV_TILE + kk;
                             const bool see = valid && tree_sees(p, mask, node, key - sg.past);
                             const uint16_t* vr = reinterpret_cast<const uint16_t*>(
                                 p.v + (sg.seq * p.kv_seq + sg.head * p.kv_head + key * p.kv_row) * 2);
+#pragma unroll 1
                             for (int c = 0; c < HD / 32; ++c) {
                                 uint32_t o[32];
                                 tmem_ld32(t_o + 32 * c, o);
@@ -434,12 +452,12 @@ __global__ void __launch_bounds__(XT, 1)
             ord += n - min(n, first_tail);
             // ---- the unit's rows, or this group's part of them
             if (mine) {
-                if (!(ok = wait_all(ms.pv_done[w], (done - 1) & 1))) break;
+                if (!(ok = wait_all(ms.pv_done[w], 1))) break;  // two phases a tile: the last one is odd
                 tc_after_sync();
             }
             const bool whole = sg.t0 == 0 && sg.t1 == sg.tiles;
             const size_t orow = ((size_t)sg.seq * p.n_nodes + node) * p.n_heads + sg.head * p.group + head_in;
-            float* part = parts + ((size_t)blockIdx.x * 2 + (sg.t0 == 0 ? 1 : 0)) * part_floats(p.block_rows, HD);
+            float* part = ws.parts + ((size_t)blockIdx.x * 2 + (sg.t0 == 0 ? 1 : 0)) * part_floats(p.block_rows, HD);
             const bool join = !two && n > 1;
             float* js = reinterpret_cast<float*>(sm);  // [128][HD], 16-byte chunk c of row r at c ^ (r & 7), over Q
             float f0 = 1.f, f1 = 0.f;
@@ -447,6 +465,7 @@ __global__ void __launch_bounds__(XT, 1)
                 if (!(ok = meet())) break;  // both groups' MMAs over Q are done
                 if (w == 1) {
                     if (warp_on) {
+#pragma unroll 1
                         for (int c = 0; c < HD / 32; ++c) {
                             uint32_t o[32];
                             tmem_ld32(t_o + 32 * c, o);
@@ -471,7 +490,8 @@ __global__ void __launch_bounds__(XT, 1)
                 }
             }
             if (warp_on && (two || w == 0)) {
-                const float inv = whole ? (l > 0.f ? 1.f / l : l == 0.f ? 1.f : l) : 1.f;  // an empty row stays 0
+                const float inv = whole ? row_inv(l) : 1.f;
+#pragma unroll 1
                 for (int c = 0; c < HD / 32; ++c) {
                     uint32_t o[32];
                     tmem_ld32(t_o + 32 * c, o);
@@ -515,8 +535,11 @@ __global__ void __launch_bounds__(XT, 1)
                     }
                 }
             }
-            if (join && !(ok = meet())) break;  // Q's memory is free again
             tc_before_sync();
+            if (w == 0) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                arrive_warp(ms.q_free);
+            }
         }
     }
     tc_before_sync();
@@ -525,33 +548,33 @@ __global__ void __launch_bounds__(XT, 1)
         tc_after_sync();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
-    pdl_trigger();
+    join_units<BF, HD, XT>(p, ms.plan, group, block, out, lse, ws);
 }
 
-bool make_map(CUtensorMap* map, const void* base, const TreeParams& p, int hd, bool bf) {
+// A map of 16-bit rows [d3][d2][d1][hd], copied in boxes of 64 columns x b1 x b2. The stride of an
+// axis of one element is never used.
+bool make_map(CUtensorMap* map, const void* base, bool bf, int hd, int64_t d1, int64_t s1, int64_t d2, int64_t s2, int64_t d3,
+              int64_t s3, int b1, int b2) {
     EncodeTiledFn enc = encode_tiled();
     if (!enc) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)p.max_ctx, (cuuint64_t)p.n_kv_heads, (cuuint64_t)p.n_seqs};
-    // the stride of an axis of one element is never used
-    const cuuint64_t strides[3] = {(cuuint64_t)(p.max_ctx > 1 ? p.kv_row * 2 : 256),
-                                   (cuuint64_t)(p.n_kv_heads > 1 ? p.kv_head * 2 : 256),
-                                   (cuuint64_t)(p.n_seqs > 1 ? p.kv_seq * 2 : 256)};
-    const cuuint32_t box[4] = {64, (cuuint32_t)KV_TILE, 1, 1}, estr[4] = {1, 1, 1, 1};
+    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3};
+    const cuuint64_t strides[3] = {(cuuint64_t)(d1 > 1 ? s1 * 2 : 256), (cuuint64_t)(d2 > 1 ? s2 * 2 : 256),
+                                   (cuuint64_t)(d3 > 1 ? s3 * 2 : 256)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, estr[4] = {1, 1, 1, 1};
     return enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
                strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <bool BF, int HD>
-cudaError_t launch_mma(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, float* parts, int* err,
-                       cudaStream_t s) {
-    CUtensorMap mk, mv;
-    if (!make_map(&mk, p.k, p, HD, BF) || !make_map(&mv, p.v, p, HD, BF)) return cudaErrorInvalidValue;
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_tree_mma<BF, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, MmaSmem<HD>::TOTAL);
-    if (e != cudaSuccess) return e;
-    k_tree_mma<BF, HD><<<plan.n_groups * plan.row_blocks, XT, MmaSmem<HD>::TOTAL, s>>>(mk, mv, p, out, lse, parts, err);
-    return cudaGetLastError();
+cudaError_t launch_mma(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, void* ws, cudaStream_t s) {
+    CUtensorMap mq, mk, mv;
+    if (!make_map(&mq, p.q, BF, HD, p.n_heads, HD, p.n_nodes, p.q_node, p.n_seqs, p.q_seq, p.group, p.tile_nodes) ||
+        !make_map(&mk, p.k, BF, HD, p.max_ctx, p.kv_row, p.n_kv_heads, p.kv_head, p.n_seqs, p.kv_seq, KV_TILE, 1) ||
+        !make_map(&mv, p.v, BF, HD, p.max_ctx, p.kv_row, p.n_kv_heads, p.kv_head, p.n_seqs, p.kv_seq, KV_TILE, 1))
+        return cudaErrorInvalidValue;
+    return launch_coop(k_tree_mma<BF, HD>, plan.n_groups * plan.row_blocks, XT, MmaSmem<HD>::TOTAL, s, mq, mk, mv, p, out, lse,
+                       ws);
 }
 
 }  // namespace
@@ -562,10 +585,9 @@ bool tree_mma_fits(const jinf_b200_kv* kv) {
 }
 
 cudaError_t tree_mma_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, uint16_t* out, float* lse,
-                            float* parts, int* err, cudaStream_t s) {
-    if (head_dim == 64)
-        return bf ? launch_mma<true, 64>(p, plan, out, lse, parts, err, s) : launch_mma<false, 64>(p, plan, out, lse, parts, err, s);
-    return bf ? launch_mma<true, 128>(p, plan, out, lse, parts, err, s) : launch_mma<false, 128>(p, plan, out, lse, parts, err, s);
+                            void* ws, cudaStream_t s) {
+    if (head_dim == 64) return bf ? launch_mma<true, 64>(p, plan, out, lse, ws, s) : launch_mma<false, 64>(p, plan, out, lse, ws, s);
+    return bf ? launch_mma<true, 128>(p, plan, out, lse, ws, s) : launch_mma<false, 128>(p, plan, out, lse, ws, s);
 }
 
 }  // namespace jinf

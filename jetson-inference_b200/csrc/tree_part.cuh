@@ -1,26 +1,156 @@
-// Partial rows of a unit that several CTAs share (tree_attn.cu, tree_mma.cu). A CTA keeps up to two:
-// slot 0 of a unit that an earlier CTA began, slot 1 of one that it begins and hands on. A slot:
+// Units that several CTAs share (tree_attn.cu, tree_mma.cu): their partial rows and the join.
+//
+// A CTA keeps up to two partial blocks: slot 0 of a unit that an earlier group of CTAs began, slot 1
+// of one that it begins and hands on. A slot:
 //   float4 [head_dim / 4][block_rows]   O, unnormalised, of scale e^-m (rows innermost: a thread
 //                                       per row writes, and the join reads, whole lines)
 //   float  [block_rows]                 m, the maximum of the unscaled scores (or a bound within 2^8)
 //   float  [block_rows]                 l
-// The workspace is the error word (256 bytes) and the slots of every CTA.
+// The join runs at the end of the same launch, whose CTAs are all resident (cooperative launch, one
+// per SM): each CTA announces its parts, waits for those of its units and joins one slice of the
+// unit's values, so that the parts are read back by as many CTAs as wrote them, and from L2. A
+// kernel of its own for it took 5 to 8 us more a call.
+// Workspace: the error word (256 bytes), a counter per CTA, the slots.
 #pragma once
 
-#include <cuda_runtime.h>
-#include <stddef.h>
+#include "kv_ops.cuh"
 
 namespace jinf {
 
 constexpr size_t TREE_WS_HEAD = 256;
+constexpr int JOIN_SPIN = 1 << 21;  // polls of a counter before the wait gives up
 
 __host__ __device__ __forceinline__ size_t part_floats(int block_rows, int hd) {
     return ((size_t)block_rows * (hd + 2) + 3) & ~(size_t)3;  // slots start on 16 bytes
 }
 
-struct TreeParams;
-struct TreePlan;
+struct TreeWs {
+    int* err;
+    unsigned* count;  // [CTAs] of the unit that CTA c begins: n parts announced, then n times seen, then 0 again
+    float* parts;
+};
+__host__ __device__ __forceinline__ size_t tree_ws_head(int n_ctas) {  // bytes before the slots
+    return TREE_WS_HEAD + (((size_t)n_ctas * 4 + 255) & ~(size_t)255);
+}
+__host__ __device__ __forceinline__ TreeWs tree_ws(void* ws, int n_ctas) {
+    TreeWs w;
+    w.err = (int*)ws;
+    w.count = (unsigned*)((uint8_t*)ws + TREE_WS_HEAD);
+    w.parts = (float*)((uint8_t*)ws + tree_ws_head(n_ctas));
+    return w;
+}
+
+template <bool BF>
+__device__ __forceinline__ void store4(uint16_t* at, float4 a, float inv) {
+    *reinterpret_cast<uint2*>(at) = make_uint2(pack2<BF>(a.x * inv, a.y * inv), pack2<BF>(a.z * inv, a.w * inv));
+}
+// 1 / l of a row; an empty row (l = 0) keeps its 0, NaN stays NaN
+__device__ __forceinline__ float row_inv(float l) { return l > 0.f ? 1.f / l : l == 0.f ? 1.f : l; }
+
+struct JoinPlan {
+    SharedUnit unit[2];
+    int n, ok[2];
+};
+// Joins the CTA's shared units, found in `plan` before (shared memory). Every thread of the CTA calls
+// it, after the CTA's parts are written. With two units each takes half of the threads. Waits are
+// bounded: one that runs out sets the error word and leaves its slice unwritten.
+template <bool BF, int HD, int THREADS>
+__device__ __forceinline__ void join_units(const TreeParams& p, JoinPlan& plan, int group, int block, uint16_t* out,
+                                           float* lse, const TreeWs& ws) {
+    __syncthreads();  // the parts are written (and visible to the others by the fence below)
+    const int n_units = plan.n;
+    if (n_units == 0) return;
+    const int half = THREADS / n_units, x = threadIdx.x / half, t = threadIdx.x - x * half;
+    const SharedUnit u = plan.unit[x];
+    const int n_parts = u.g1 - u.g0 + 1;
+    unsigned* count = ws.count + u.g0 * p.row_blocks + block;
+    if (t == 0) {
+        __threadfence();
+        atomicInc(count, 2 * n_parts - 1);
+        int ok = 0;
+        for (int it = 0; it < JOIN_SPIN && !ok; ++it) {
+            unsigned v;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(count) : "memory");
+            ok = v >= (unsigned)n_parts;
+        }
+        // seen: the last one to see wraps the counter to 0, for the next launch
+        if (ok) atomicInc(count, 2 * n_parts - 1);
+        else atomicExch(ws.err, 1);
+        plan.ok[x] = ok;
+    }
+    __syncthreads();
+    if (!plan.ok[x]) return;
+    const int row0 = block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
+    const uint32_t pf4 = (uint32_t)(part_floats(p.block_rows, HD) / 4);
+    const float c2 = p.scale * LOG2E;
+    const int items = rows * (HD / 4), mine = group - u.g0;
+    const int i1 = items * (mine + 1) / n_parts;
+    const float4* parts = reinterpret_cast<const float4*>(ws.parts) + (size_t)((u.g0 * p.row_blocks + block) * 2) * pf4;
+    for (int i = items * mine / n_parts + t; i < i1; i += half) {
+        const int d4 = i / rows, r = i - d4 * rows;
+        float M = -INFINITY, L = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int B = 12;
+        for (int kb = 0; kb < n_parts; kb += B) {  // in the groups' order, twelve parts in flight
+            float pm[B], pl[B];
+            float4 po[B];
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                pm[k] = -INFINITY;
+                pl[k] = 0.f;
+                po[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (kb + k < n_parts) {
+                    // the group that begins the unit kept it in its second slot, the others in their first
+                    const float4* part = parts + (size_t)((kb + k) * 2 * p.row_blocks + (kb + k == 0)) * pf4;
+                    const float* ml = reinterpret_cast<const float*>(part + p.block_rows * (HD / 4)) + r;
+                    pm[k] = __ldcg(ml);
+                    pl[k] = __ldcg(ml + p.block_rows);
+                    po[k] = __ldcg(part + d4 * p.block_rows + r);
+                }
+            }
+            float mn = M;
+#pragma unroll
+            for (int k = 0; k < B; ++k) mn = fmaxf(mn, pm[k]);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float corr = exp2f((M - base) * c2);
+            M = mn;
+            L *= corr;
+            a.x *= corr; a.y *= corr; a.z *= corr; a.w *= corr;
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const float f = exp2f((pm[k] - base) * c2);
+                L = fmaf(pl[k], f, L);
+                a.x = fmaf(po[k].x, f, a.x);
+                a.y = fmaf(po[k].y, f, a.y);
+                a.z = fmaf(po[k].z, f, a.z);
+                a.w = fmaf(po[k].w, f, a.w);
+            }
+        }
+        const int rr = row0 + r;
+        const size_t orow = ((size_t)u.seq * p.n_nodes + rr / p.group) * p.n_heads + u.head * p.group + rr % p.group;
+        store4<BF>(out + orow * HD + d4 * 4, a, row_inv(L));
+        if (lse && d4 == 0) lse[orow] = L == 0.f ? -INFINITY : M * p.scale + logf(L);
+    }
+}
+
+template <typename K, typename... A>
+cudaError_t launch_coop(K kernel, int grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeCooperative;
+    attr[0].val.cooperative = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 cudaError_t tree_mma_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, uint16_t* out, float* lse,
-                            float* parts, int* err, cudaStream_t s);
+                            void* ws, cudaStream_t s);
 
 }  // namespace jinf

@@ -40,6 +40,13 @@ __device__ __forceinline__ bool mb_wait(uint32_t b, uint32_t parity) {
     return false;
 }
 
+// true in one lane of a converged warp, always the same one
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.b32 %0, 1, 0, p; }" : "=r"(e));
+    return e;
+}
+
 // raw bytes global -> shared on an mbarrier (16-byte aligned, a multiple of 16 bytes)
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),

@@ -69,7 +69,8 @@ def mass(kv, **kw):
 
 QUERY = [dict(q=None), dict(q=P + 8), dict(qs=1023), dict(qn=516), dict(nh=3), dict(nh=0), dict(nodes=0),
          dict(nodes=257), dict(n_past=None), dict(max_past=98), dict(max_past=-1), dict(ms=-1), dict(scale=0.0),
-         dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))]
+         dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(qs=0), dict(qn=0), dict(qn=-512),
+         dict(qs=1 << 39)]
 
 
 @pytest.mark.parametrize("bad", BAD_VIEWS)
@@ -130,6 +131,15 @@ def commit(kv, **kw):
 def test_tree_commit_refuses(bad):
     assert commit(view(), **bad) == INVALID
     assert commit(None) == INVALID
+
+
+def test_more_than_64_query_heads_per_kv_head_are_refused():
+    assert tree(view(), nh=130, max_past=0) == INVALID and mass(view(), nh=130, max_past=0) == INVALID
+
+
+def test_more_than_2_31_key_tiles_are_refused():
+    kv = view(n_seqs=1024, n_kv_heads=65535, max_ctx=1 << 30, seq_stride=0, head_stride=0)
+    assert tree(kv, nh=65535, max_past=(1 << 30) - 3) == INVALID and mass(kv, nh=65535, max_past=(1 << 30) - 3) == INVALID
 
 
 def test_workspace_is_bounded_by_the_device_not_by_the_context():
