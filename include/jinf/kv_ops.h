@@ -68,8 +68,7 @@ jinf_status jinf_b200_tree_mask(const int32_t* parents, int n_nodes, uint32_t* m
 // n_past: device int32 [n_seqs], each clamped to 0..max_past; max_past + n_nodes <= max_ctx.
 // scale > 0. workspace (16-byte aligned): tree_attention_workspace_bytes for the same arguments,
 // zeroed once before first use, then reusable on the same stream; calls that overlap in time need
-// one each. Its first int32 becomes 1 if a wait inside the kernel ran out (the output is then
-// incomplete, and the workspace is to be zeroed again).
+// one each.
 size_t jinf_b200_tree_attention_workspace_bytes(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past);
 jinf_status jinf_b200_tree_attention(void* out, float* lse, const void* q, int64_t q_seq_stride,
                                      int64_t q_node_stride, int n_heads, int n_nodes, const jinf_b200_kv* kv,
@@ -109,6 +108,11 @@ jinf_status jinf_b200_kv_evict(const jinf_b200_kv* kv, const jinf_b200_kv* kv_ou
 jinf_status jinf_b200_tree_commit(const jinf_b200_kv* kv, float* mass, const int32_t* n_past, int max_past,
                                   const int32_t* accepted, int accepted_stride, const int32_t* n_accepted, int n_nodes,
                                   int32_t* n_out, cudaStream_t stream);
+
+// The kernels' waits inside a launch are bounded. JINF_ERR_TIMEOUT if one of the current device's ran
+// out since the last call (outputs since then are incomplete, and tree-attention workspaces are to be
+// zeroed again), else JINF_OK. Synchronises with the default stream.
+jinf_status jinf_b200_kv_ops_status(void);
 
 #ifdef __cplusplus
 }

@@ -14,6 +14,7 @@
 namespace jinf {
 namespace {
 
+constexpr int MASS_MMA_ROWS = 16;  // more query rows go to k_mass_mma (mass_mma.cu)
 constexpr int MW = 8;        // warps of a CTA, 16 keys each
 constexpr int MROWS = 32;    // query rows of a stage
 static_assert(MW * 16 == KV_TILE, "a CTA owns one tile of keys");
@@ -163,8 +164,9 @@ cudaError_t launch_mass(const TreeParams& p, const float* lse, const float* weig
 
 }  // namespace
 
-cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, const float* lse, const float* weight,
-                             float* mass, cudaStream_t s) {
+cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, bool map_fits, const float* lse,
+                             const float* weight, float* mass, cudaStream_t s) {
+    if (map_fits && p.n_rows > MASS_MMA_ROWS) return mass_mma_launch(p, bf, head_dim, lse, weight, mass, s);
     if (head_dim == 64) return bf ? launch_mass<true, 64>(p, lse, weight, mass, s) : launch_mass<false, 64>(p, lse, weight, mass, s);
     return bf ? launch_mass<true, 128>(p, lse, weight, mass, s) : launch_mass<false, 128>(p, lse, weight, mass, s);
 }

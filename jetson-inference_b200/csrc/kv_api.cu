@@ -20,7 +20,37 @@ int kv_device_sms() {
     }
     return n;
 }
+
+bool kv_map_fits(const jinf_b200_kv* kv) {
+    auto ok = [](int n, int64_t stride) { return n == 1 || (stride > 0 && stride * 2 < ((int64_t)1 << 40)); };
+    return ok(kv->max_ctx, kv->row_stride) && ok(kv->n_kv_heads, kv->head_stride) && ok(kv->n_seqs, kv->seq_stride);
+}
 }  // namespace jinf
+
+// Set by a bounded wait that ran out, in any of the kernels.
+static __device__ int g_kv_error;
+
+static int* error_word() {
+    static std::atomic<int*> addr[64];  // per device; every writer stores the same address
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    int* a = addr[dev].load(std::memory_order_acquire);
+    if (!a) {
+        void* p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_kv_error) != cudaSuccess) return nullptr;
+        a = (int*)p;
+        addr[dev].store(a, std::memory_order_release);
+    }
+    return a;
+}
+
+extern "C" jinf_status jinf_b200_kv_ops_status(void) {
+    int e = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(&e, g_kv_error, sizeof(e)) != cudaSuccess) return JINF_ERR_CUDA;
+    if (e && cudaMemcpyToSymbol(g_kv_error, &zero, sizeof(zero)) != cudaSuccess) return JINF_ERR_CUDA;
+    return e ? JINF_ERR_TIMEOUT : JINF_OK;
+}
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -42,7 +72,7 @@ static bool tree_shape_ok(const jinf_b200_kv* kv, int n_heads, int n_nodes, int 
 
 static TreePlan plan_of(const jinf_b200_kv* kv, int n_heads, int n_nodes, int max_past) {
     return tree_plan(kv->n_seqs, kv->n_kv_heads, n_heads / kv->n_kv_heads, n_nodes, max_past, kv_device_sms(),
-                     tree_mma_fits(kv));
+                     kv_map_fits(kv));
 }
 
 static void tree_params(TreeParams* p, const void* q, int64_t q_seq, int64_t q_node, int n_heads, int n_nodes,
@@ -111,6 +141,7 @@ extern "C" jinf_status jinf_b200_tree_attention(void* out, float* lse, const voi
     TreeParams p;
     tree_params(&p, q, q_seq_stride, q_node_stride, n_heads, n_nodes, kv, n_past, max_past, mask, mask_seq_stride, scale);
     const TreePlan plan = plan_of(kv, n_heads, n_nodes, max_past);
+    if (!(p.err = error_word())) return JINF_ERR_CUDA;
     p.row_blocks = plan.row_blocks;
     p.block_rows = plan.block_rows;
     return tree_attn_launch(p, plan, kv->type == JINF_B200_BF16, kv->head_dim, out, lse, workspace, stream) ==
@@ -129,7 +160,9 @@ extern "C" jinf_status jinf_b200_attention_mass(float* mass, const void* q, int6
         return JINF_ERR_INVALID;
     TreeParams p;
     tree_params(&p, q, q_seq_stride, q_node_stride, n_heads, n_nodes, kv, n_past, max_past, mask, mask_seq_stride, scale);
-    return attn_mass_launch(p, kv->type == JINF_B200_BF16, kv->head_dim, lse, node_weight, mass, stream) == cudaSuccess
+    if (!(p.err = error_word())) return JINF_ERR_CUDA;
+    return attn_mass_launch(p, kv->type == JINF_B200_BF16, kv->head_dim, kv_map_fits(kv), lse, node_weight, mass, stream) ==
+                   cudaSuccess
                ? JINF_OK
                : JINF_ERR_CUDA;
 }

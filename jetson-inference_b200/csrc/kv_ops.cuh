@@ -4,6 +4,7 @@
 
 #include "common.cuh"
 #include "mma_f16.cuh"
+#include "umma.cuh"
 #include "jinf/kv_ops.h"
 
 #include <cuda_bf16.h>
@@ -29,6 +30,7 @@ struct TreeParams {
     int block_rows;  // rows of a block (the last may have fewer)
     int tile_nodes;  // k_tree_mma: nodes whose rows fill one tile of 128 query rows
     float scale;
+    int* err;  // set to 1 by a wait that ran out (jinf_b200_kv_ops_status)
 };
 
 __device__ __forceinline__ int clamped_past(const TreeParams& p, int seq) {
@@ -38,6 +40,22 @@ __device__ __forceinline__ int clamped_past(const TreeParams& p, int seq) {
 // Whether node t sees tree row u (both < n_nodes); `mask`: the sequence's words or null.
 __device__ __forceinline__ bool tree_sees(const TreeParams& p, const uint32_t* mask, int t, int u) {
     return mask ? (mask[t * p.mask_words + (u >> 5)] >> (u & 31)) & 1u : u <= t;
+}
+
+// Tree rows 32 w .. 32 w + 31 that node t sees, as bits.
+__device__ __forceinline__ uint32_t seen_word(const TreeParams& p, const uint32_t* mask, int t, int w) {
+    if (w < 0 || w >= p.mask_words) return 0u;
+    const int left = p.n_nodes - 32 * w;
+    uint32_t x;
+    if (mask) x = mask[t * p.mask_words + w];
+    else x = t >= 32 * w + 31 ? 0xFFFFFFFFu : t < 32 * w ? 0u : (2u << (t - 32 * w)) - 1u;
+    return left >= 32 ? x : x & ((1u << left) - 1u);
+}
+// Keys whose first is tree row u0 (negative: -u0 cached rows come first), 32 of them, as bits.
+__device__ __forceinline__ uint32_t seen_keys(const TreeParams& p, const uint32_t* mask, int t, int u0) {
+    if (u0 <= -32) return 0xFFFFFFFFu;
+    if (u0 < 0) return (seen_word(p, mask, t, 0) << (-u0)) | ((1u << (-u0)) - 1u);
+    return __funnelshift_r(seen_word(p, mask, t, u0 >> 5), seen_word(p, mask, t, (u0 >> 5) + 1), u0 & 31);
 }
 
 template <bool BF>
@@ -59,6 +77,12 @@ template <bool BF>
 __device__ __forceinline__ bool nonfinite2(uint32_t w) {
     constexpr uint32_t E = BF ? 0x7F80u : 0x7C00u;
     return (w & E) == E || ((w >> 16) & E) == E;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // c += A B, m16n8k16, fp32 accumulators
@@ -209,6 +233,11 @@ __device__ __forceinline__ int shared_units(const TreeParams& p, int g, const Sh
 
 int kv_device_sms();  // SMs of the current device (cached per device)
 
+// Key tiles of K or V, [seq][head][row][hd], as boxes of 64 columns x KV_TILE rows
+inline bool kv_tile_map(CUtensorMap* map, const void* base, const TreeParams& p, bool bf, int hd) {
+    return rows_map(map, base, bf, hd, p.max_ctx, p.kv_row, p.n_kv_heads, p.kv_head, p.n_seqs, p.kv_seq, KV_TILE, 1);
+}
+
 // ---- launches (return a cudaError_t; arguments already checked) ----
 
 struct TreePlan {
@@ -218,13 +247,15 @@ struct TreePlan {
 };
 TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_past, int sms, bool mma_fits);
 size_t tree_workspace_bytes(const TreePlan& plan, int head_dim);
-// k_tree_mma's tensor maps describe this cache (their strides are below 2^40 bytes and not 0)
-bool tree_mma_fits(const jinf_b200_kv* kv);
+// tensor maps can describe this cache (strides below 2^40 bytes and not 0)
+bool kv_map_fits(const jinf_b200_kv* kv);
 cudaError_t tree_attn_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, void* out, float* lse,
                              void* ws, cudaStream_t s);
 
-cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, const float* lse, const float* weight,
+cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, bool map_fits, const float* lse, const float* weight,
                              float* mass, cudaStream_t s);
+cudaError_t mass_mma_launch(const TreeParams& p, bool bf, int head_dim, const float* lse, const float* weight, float* mass,
+                            cudaStream_t s);
 
 struct KvPlanes {  // K and V with their strides in bytes
     uint8_t* k;

@@ -19,7 +19,7 @@
 // The accumulator is rescaled only when a row's maximum has grown by more than 2^8 since the last
 // time: p is at most 2^8 then, which both 16-bit types and the fp32 sums hold with the precision
 // that they have for p <= 1, and the rescaling (a read and a write of all of O) almost never runs.
-// Every wait is bounded; one that runs out sets the workspace's error word and ends the CTA.
+// Every wait is bounded; one that runs out sets the error word and ends the CTA.
 #include "kv_ops.cuh"
 #include "tree_part.cuh"
 #include "umma.cuh"
@@ -42,7 +42,7 @@ struct MmaSmem {
     static constexpr int OFF_MISC = OFF_KV + ST * TILE;
     struct Misc {
         uint64_t full[ST], empty[ST], vok[BAD_SETS];
-        uint64_t s_full[2][2], p_ready[2][2], pv_done[2], flag_ok[2], drain[2], join, q_full, q_free;
+        uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2], flag_ok[2], drain[2], join, q_full, q_free;
         Share share;
         Shares all;
         JoinPlan plan;
@@ -54,28 +54,6 @@ struct MmaSmem {
     static constexpr int TOTAL = OFF_MISC + (int)sizeof(Misc) + 1024;
 };
 static_assert(MmaSmem<128>::TOTAL + 256 <= 232448 && MmaSmem<64>::TOTAL + 256 <= 232448, "shared memory (with join_units')");
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Tree rows 32 w .. 32 w + 31 that node t sees, as bits.
-__device__ __forceinline__ uint32_t seen_word(const TreeParams& p, const uint32_t* mask, int t, int w) {
-    if (w < 0 || w >= p.mask_words) return 0u;
-    const int left = p.n_nodes - 32 * w;
-    uint32_t x;
-    if (mask) x = mask[t * p.mask_words + w];
-    else x = t >= 32 * w + 31 ? 0xFFFFFFFFu : t < 32 * w ? 0u : (2u << (t - 32 * w)) - 1u;
-    return left >= 32 ? x : x & ((1u << left) - 1u);
-}
-// Keys whose first is tree row u0 (negative: -u0 cached rows come first), 32 of them, as bits.
-__device__ __forceinline__ uint32_t seen_keys(const TreeParams& p, const uint32_t* mask, int t, int u0) {
-    if (u0 <= -32) return 0xFFFFFFFFu;
-    if (u0 < 0) return (seen_word(p, mask, t, 0) << (-u0)) | ((1u << (-u0)) - 1u);
-    return __funnelshift_r(seen_word(p, mask, t, u0 >> 5), seen_word(p, mask, t, (u0 >> 5) + 1), u0 & 31);
-}
 
 template <bool BF, int HD>
 __global__ void __launch_bounds__(XT, 1)
@@ -99,15 +77,15 @@ __global__ void __launch_bounds__(XT, 1)
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
             mb_init(su32(&ms.full[i]), 1);
-            mb_init(su32(&ms.empty[i]), two ? 2 : 1);  // a tile is used by both groups, or by one
+            mb_init(su32(&ms.empty[i]), (two ? 2 : 1) + 1);  // both groups' issuers, or one, and the cleaner
         }
         for (int i = 0; i < BAD_SETS; ++i) mb_init(su32(&ms.vok[i]), 1);
         for (int w = 0; w < 2; ++w) {
             for (int h = 0; h < 2; ++h) {
                 mb_init(su32(&ms.s_full[w][h]), 1);
                 mb_init(su32(&ms.p_ready[w][h]), 4);
+                mb_init(su32(&ms.pv_done[w][h]), 1);
             }
-            mb_init(su32(&ms.pv_done[w]), 1);
             mb_init(su32(&ms.flag_ok[w]), 1);
             mb_init(su32(&ms.drain[w]), 1);
         }
@@ -136,6 +114,10 @@ __global__ void __launch_bounds__(XT, 1)
     Share share = ms.share;
     Segment sg;
 
+    // A wait by parity tells phase x only from x - 1 and x + 1: a thread that waits for phase x of a
+    // barrier must know that x - 1 is over and that x + 1 is not. So each role waits for every
+    // phase of a barrier in order (or for one whose predecessor an earlier wait implies), and no phase
+    // ends twice before it has looked.
     // a bounded wait that also ends when another role gave up
     auto wait = [&](uint64_t& bar, uint32_t parity) -> bool {
         const uint32_t b = su32(&bar);
@@ -144,7 +126,7 @@ __global__ void __launch_bounds__(XT, 1)
             if ((it & 255) == 255 && *(volatile int*)&ms.abort) return false;
         }
         atomicExch(&ms.abort, 1);
-        atomicExch(ws.err, 1);
+        atomicExch(p.err, 1);
         return false;
     };
     // the same for a whole warp, which stays converged
@@ -161,6 +143,8 @@ __global__ void __launch_bounds__(XT, 1)
     // order in which the MMAs take them), the last V_i without a K.
     auto pos_k = [](int i) { return i ? 2 * i - 1 : 0; };
     auto pos_v = [](int i, int n) { return i + 1 < n ? 2 * i + 2 : 2 * n - 1; };
+    auto k_at = [](int x, int n) { return x == 0 || ((x & 1) && x < 2 * n - 1); };  // position x holds a K
+    auto tile_at = [](int x, int n) { return x == 2 * n - 1 ? n - 1 : x & 1 ? (x + 1) / 2 : x ? x / 2 - 1 : 0; };
 
     if (warp == 0) {
         if (lane == 0) {  // ---- copies
@@ -179,9 +163,8 @@ __global__ void __launch_bounds__(XT, 1)
                                     row0 / p.group + w * p.tile_nodes, sg.seq, qbar);
                 ++units;
                 for (int x = 0; ok && x < 2 * n; ++x, ++pos) {
-                    // x-th of the order above
-                    const bool is_k = x == 0 || ((x & 1) && x < 2 * n - 1);
-                    const int i = x == 0 ? 0 : is_k ? (x + 1) / 2 : x == 2 * n - 1 ? n - 1 : x / 2 - 1;
+                    const bool is_k = k_at(x, n);
+                    const int i = tile_at(x, n);
                     const uint32_t slot = pos % ST, fill = pos / ST;
                     if (fill && !(ok = wait(ms.empty[slot], (fill - 1) & 1))) break;
                     const uint32_t bar = su32(&ms.full[slot]);
@@ -203,9 +186,13 @@ __global__ void __launch_bounds__(XT, 1)
         const bool leader = elect_one();
         const uint32_t t_s = tmem + 128 * w, t_o = tmem + 256 + 128 * w;
         const uint64_t dq = umma_desc(s_q + (two ? w : 0) * TILE);
-        uint32_t base = 0, done = 0, units = 0, ord = 0;
+        uint32_t base = 0, done = 0, units = 0, ord = 0, landed = 0;
         bool ok = true;
-        auto full = [&](uint32_t pos) { return wait_all(ms.full[pos % ST], (pos / ST) & 1); };
+        auto full = [&](uint32_t pos) {  // the tiles up to ring position pos
+            for (; landed <= pos; ++landed)
+                if (!wait_all(ms.full[landed % ST], (landed / ST) & 1)) return false;
+            return true;
+        };
         auto qk = [&](uint32_t pos, int h) {
             const uint64_t dk = umma_desc(s_kv + (pos % ST) * TILE + h * 8192);
 #pragma unroll
@@ -218,9 +205,10 @@ __global__ void __launch_bounds__(XT, 1)
         while (ok && share.next(p, sg)) {
             const int n = sg.t1 - sg.t0, first_tail = max(0, sg.past / KV_TILE - sg.t0);
             int i = two ? 0 : w;
+            if (!(ok = wait_all(ms.q_full, units & 1))) break;
             if (i < n) {
                 const uint32_t k = base + pos_k(i);
-                if (!(ok = wait_all(ms.q_full, units & 1) && full(k))) break;
+                if (!(ok = full(k))) break;
                 tc_after_sync();
                 if (leader) {
                     qk(k, 0);
@@ -247,7 +235,7 @@ __global__ void __launch_bounds__(XT, 1)
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
                             umma_ts(t_o, t_s + 64 * h + 8 * kk, dv + ((4 * h + kk) * 2048 >> 4), ID_PV, i >= step || h || kk > 0);
-                        umma_commit(su32(&ms.pv_done[w]));
+                        umma_commit(su32(&ms.pv_done[w][h]));
                         if (h == 1) umma_commit(su32(&ms.empty[v % ST]));
                         if (more) qk(k, h);
                         if (more && h == 1) umma_commit(su32(&ms.empty[k % ST]));
@@ -279,13 +267,18 @@ __global__ void __launch_bounds__(XT, 1)
                 ms.plan.unit[1] = u[1];
             }
         }
-        uint32_t base = 0, ord = 0;
+        // It sees every tile land, in order, and a slot is not filled again before it has.
+        uint32_t pos = 0, ord = 0;
         bool ok = true;
         while (ok && share.next(p, sg)) {
             const int n = sg.t1 - sg.t0, n_keys = sg.past + p.n_nodes;
-            for (int i = max(0, sg.past / KV_TILE - sg.t0); i < n; ++i, ++ord) {
-                const uint32_t pos = base + pos_v(i, n);
+            for (int at = 0; at < 2 * n; ++at, ++pos) {
                 if (!(ok = wait_all(ms.full[pos % ST], (pos / ST) & 1))) break;
+                const int i = tile_at(at, n);
+                if (k_at(at, n) || (sg.t0 + i + 1) * KV_TILE <= sg.past) {
+                    arrive_warp(ms.empty[pos % ST]);
+                    continue;
+                }
                 uint32_t* bad = ms.bad[ord % BAD_SETS];
                 if (lane < 4) bad[lane] = 0;
                 __syncwarp();
@@ -313,8 +306,9 @@ __global__ void __launch_bounds__(XT, 1)
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 arrive_warp(ms.vok[ord % BAD_SETS]);
+                arrive_warp(ms.empty[pos % ST]);
+                ++ord;
             }
-            base += 2 * n;
         }
     } else {
         // ---- softmax groups
@@ -379,7 +373,8 @@ __global__ void __launch_bounds__(XT, 1)
                                 const float f = need ? ex2((m - mx) * c2) : 1.f;
                                 if (need) m = mx;
                                 l *= f;
-                                ok = wait_all(ms.pv_done[w], (2 * done + h - 1) & 1);
+                                // the previous half's P V; the one before it was over before these scores came
+                                ok = h ? wait_all(ms.pv_done[w][0], done & 1) : wait_all(ms.pv_done[w][1], (done - 1) & 1);
                                 tc_after_sync();
 #pragma unroll 1
                                 for (int c = 0; c < HD / 32; ++c) {
@@ -421,7 +416,7 @@ __global__ void __launch_bounds__(XT, 1)
                     if (!(ok = wait_all(ms.flag_ok[w], tails++ & 1))) break;
                     const uint32_t any = notes[0] | notes[1] | notes[2] | notes[3];
                     if (any && warp_on) {  // values that are not finite, to the rows that see their key
-                        ok = wait_all(ms.pv_done[w], 1);
+                        ok = wait_all(ms.pv_done[w][1], (done - 1) & 1);
                         tc_after_sync();
                         for (int kk = 0; kk < KV_TILE; ++kk) {
                             if (!((notes[kk >> 5] >> (kk & 31)) & 1u)) continue;
@@ -452,7 +447,7 @@ __global__ void __launch_bounds__(XT, 1)
             ord += n - min(n, first_tail);
             // ---- the unit's rows, or this group's part of them
             if (mine) {
-                if (!(ok = wait_all(ms.pv_done[w], 1))) break;  // two phases a tile: the last one is odd
+                if (!(ok = wait_all(ms.pv_done[w][1], (done - 1) & 1))) break;
                 tc_after_sync();
             }
             const bool whole = sg.t0 == 0 && sg.t1 == sg.tiles;
@@ -551,38 +546,17 @@ __global__ void __launch_bounds__(XT, 1)
     join_units<BF, HD, XT>(p, ms.plan, group, block, out, lse, ws);
 }
 
-// A map of 16-bit rows [d3][d2][d1][hd], copied in boxes of 64 columns x b1 x b2. The stride of an
-// axis of one element is never used.
-bool make_map(CUtensorMap* map, const void* base, bool bf, int hd, int64_t d1, int64_t s1, int64_t d2, int64_t s2, int64_t d3,
-              int64_t s3, int b1, int b2) {
-    EncodeTiledFn enc = encode_tiled();
-    if (!enc) return false;
-    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3};
-    const cuuint64_t strides[3] = {(cuuint64_t)(d1 > 1 ? s1 * 2 : 256), (cuuint64_t)(d2 > 1 ? s2 * 2 : 256),
-                                   (cuuint64_t)(d3 > 1 ? s3 * 2 : 256)};
-    const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, estr[4] = {1, 1, 1, 1};
-    return enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
-               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <bool BF, int HD>
 cudaError_t launch_mma(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, void* ws, cudaStream_t s) {
     CUtensorMap mq, mk, mv;
-    if (!make_map(&mq, p.q, BF, HD, p.n_heads, HD, p.n_nodes, p.q_node, p.n_seqs, p.q_seq, p.group, p.tile_nodes) ||
-        !make_map(&mk, p.k, BF, HD, p.max_ctx, p.kv_row, p.n_kv_heads, p.kv_head, p.n_seqs, p.kv_seq, KV_TILE, 1) ||
-        !make_map(&mv, p.v, BF, HD, p.max_ctx, p.kv_row, p.n_kv_heads, p.kv_head, p.n_seqs, p.kv_seq, KV_TILE, 1))
+    if (!rows_map(&mq, p.q, BF, HD, p.n_heads, HD, p.n_nodes, p.q_node, p.n_seqs, p.q_seq, p.group, p.tile_nodes) ||
+        !kv_tile_map(&mk, p.k, p, BF, HD) || !kv_tile_map(&mv, p.v, p, BF, HD))
         return cudaErrorInvalidValue;
     return launch_coop(k_tree_mma<BF, HD>, plan.n_groups * plan.row_blocks, XT, MmaSmem<HD>::TOTAL, s, mq, mk, mv, p, out, lse,
                        ws);
 }
 
 }  // namespace
-
-bool tree_mma_fits(const jinf_b200_kv* kv) {
-    auto ok = [](int n, int64_t stride) { return n == 1 || (stride > 0 && stride * 2 < ((int64_t)1 << 40)); };
-    return ok(kv->max_ctx, kv->row_stride) && ok(kv->n_kv_heads, kv->head_stride) && ok(kv->n_seqs, kv->seq_stride);
-}
 
 cudaError_t tree_mma_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, uint16_t* out, float* lse,
                             void* ws, cudaStream_t s) {

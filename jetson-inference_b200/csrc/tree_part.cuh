@@ -10,14 +10,13 @@
 // per SM): each CTA announces its parts, waits for those of its units and joins one slice of the
 // unit's values, so that the parts are read back by as many CTAs as wrote them, and from L2. A
 // kernel of its own for it took 5 to 8 us more a call.
-// Workspace: the error word (256 bytes), a counter per CTA, the slots.
+// Workspace: a counter per CTA, the slots.
 #pragma once
 
 #include "kv_ops.cuh"
 
 namespace jinf {
 
-constexpr size_t TREE_WS_HEAD = 256;
 constexpr int JOIN_SPIN = 1 << 21;  // polls of a counter before the wait gives up
 
 __host__ __device__ __forceinline__ size_t part_floats(int block_rows, int hd) {
@@ -25,17 +24,15 @@ __host__ __device__ __forceinline__ size_t part_floats(int block_rows, int hd) {
 }
 
 struct TreeWs {
-    int* err;
     unsigned* count;  // [CTAs] of the unit that CTA c begins: n parts announced, then n times seen, then 0 again
     float* parts;
 };
 __host__ __device__ __forceinline__ size_t tree_ws_head(int n_ctas) {  // bytes before the slots
-    return TREE_WS_HEAD + (((size_t)n_ctas * 4 + 255) & ~(size_t)255);
+    return ((size_t)n_ctas * 4 + 255) & ~(size_t)255;
 }
 __host__ __device__ __forceinline__ TreeWs tree_ws(void* ws, int n_ctas) {
     TreeWs w;
-    w.err = (int*)ws;
-    w.count = (unsigned*)((uint8_t*)ws + TREE_WS_HEAD);
+    w.count = (unsigned*)ws;
     w.parts = (float*)((uint8_t*)ws + tree_ws_head(n_ctas));
     return w;
 }
@@ -75,7 +72,7 @@ __device__ __forceinline__ void join_units(const TreeParams& p, JoinPlan& plan, 
         }
         // seen: the last one to see wraps the counter to 0, for the next launch
         if (ok) atomicInc(count, 2 * n_parts - 1);
-        else atomicExch(ws.err, 1);
+        else atomicExch(p.err, 1);
         plan.ok[x] = ok;
     }
     __syncthreads();

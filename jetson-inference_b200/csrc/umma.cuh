@@ -161,4 +161,19 @@ inline EncodeTiledFn encode_tiled() {
     return fn;
 }
 
+// A map of 16-bit rows [d3][d2][d1][hd], copied in boxes of 64 columns x b1 x b2. The stride of an
+// axis of one element is never used.
+inline bool rows_map(CUtensorMap* map, const void* base, bool bf, int hd, int64_t d1, int64_t s1, int64_t d2, int64_t s2, int64_t d3,
+              int64_t s3, int b1, int b2) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)d1, (cuuint64_t)d2, (cuuint64_t)d3};
+    const cuuint64_t strides[3] = {(cuuint64_t)(d1 > 1 ? s1 * 2 : 256), (cuuint64_t)(d2 > 1 ? s2 * 2 : 256),
+                                   (cuuint64_t)(d3 > 1 ? s3 * 2 : 256)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, estr[4] = {1, 1, 1, 1};
+    return enc(map, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
+               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace jinf

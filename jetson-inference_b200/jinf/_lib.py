@@ -187,6 +187,7 @@ SIGNATURES = {
     "jinf_b200_attention_mass": (i32, [vp, vp, i64, i64, i32, i32, vp, vp, i32, vp, vp, i64, vp, f32, vp]),
     "jinf_b200_kv_evict": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, vp]),
     "jinf_b200_tree_commit": (i32, [vp, vp, vp, i32, vp, i32, vp, i32, vp, vp]),
+    "jinf_b200_kv_ops_status": (i32, []),
     # gguf.h
     "jinf_gguf_open": (i32, [C.POINTER(C.POINTER(GgufFile)), C.c_char_p]),
     "jinf_gguf_close": (None, [C.POINTER(GgufFile)]),

@@ -309,3 +309,9 @@ def tree_commit(kv: KvView, mass, n_past, max_past: int, accepted, n_accepted, n
                                         accepted.shape[1],
                                         _dense(n_accepted, "n_accepted", torch.int32, (kv.n_seqs,)), n_nodes, no,
                                         _s(stream)), "jinf_b200_tree_commit")
+
+
+def kv_ops_status() -> None:
+    """Raises JinfError (timed out) if a bounded wait inside one of the operators above ran out since the
+    last call."""
+    L.check(L.lib.jinf_b200_kv_ops_status(), "jinf_b200_kv_ops_status")

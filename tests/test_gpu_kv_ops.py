@@ -448,3 +448,34 @@ def test_wrappers_refuse_what_does_not_fit(cuda):
                    torch.empty(2, 2, 51, dtype=torch.int32, device="cuda"), None, 51)
     with pytest.raises(ValueError):
         K.tree_commit(kv, None, n, 40, torch.zeros(2, dtype=torch.int32, device="cuda"), n, 3)
+
+
+@pytest.mark.parametrize("dtype,hd,nh,nkv,nodes,lengths", [
+    (F16, 128, 8, 1, 33, [40000, 17]), (BF16, 128, 4, 1, 30, [33333]), (F16, 64, 4, 2, 64, [30000, 29999, 12345])])
+def test_long_caches_many_tiles_per_cta(cuda, dtype, hd, nh, nkv, nodes, lengths):
+    """Dozens of key tiles pass through each CTA's ring, with values that are not finite behind the tree, many
+    times over: out, lse and mass stay the same bits, and the first of them right."""
+    from jinf import kernels as K
+    g = gen(31)
+    S, mp = len(lengths), max(lengths)
+    k, v = make_cache(g, S, nkv, mp + nodes + 200, hd, dtype)
+    for s, n in enumerate(lengths):
+        k[s, :, n + nodes:], v[s, :, n + nodes:] = math.nan, math.inf
+    q = torch.randn(S, nodes, nh, hd, generator=g, device="cuda", dtype=dtype) * 1.5
+    n_past = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    mask = K.tree_mask(random_parents(4, nodes)).cuda()
+    out, lse = attend(q, k, v, n_past, mp, mask)
+    check_attention(q, k, v, n_past, out, lse, [mask] * S, hd ** -0.5)
+    kv = K.KvView(k, v)
+    want, add = ref.mass(torch.zeros(S, nkv, kv.max_ctx, device="cuda"), q, k, lengths, [mask] * S, lse, None, hd ** -0.5)
+    first = None
+    ws = torch.zeros(K.tree_attention_workspace_bytes(kv, nh, nodes, mp), dtype=torch.uint8, device="cuda")
+    for _ in range(60):
+        o, e, m = torch.empty_like(out), torch.empty_like(lse), torch.zeros(S, nkv, kv.max_ctx, device="cuda")
+        K.tree_attention(o, q, kv, n_past, mp, ws, mask=mask, lse=e)
+        K.attention_mass(m, q, kv, n_past, mp, lse, mask=mask)
+        if first is None:
+            first = m
+            assert bool(((m.double() - want).abs() <= 1e-4 * add + 2.0 ** -22 * want.abs()).all())
+        assert torch.equal(o, out) and torch.equal(e, lse) and torch.equal(m, first)
+    K.kv_ops_status()
