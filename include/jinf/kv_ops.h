@@ -79,8 +79,9 @@ jinf_status jinf_b200_tree_attention(void* out, float* lse, const void* q, int64
 //   mass[s][kvh][j] = (j < n_past[s] ? mass[s][kvh][j] : 0)
 //                     + sum_t node_weight[s][t] sum_(h of kvh) e^(scale q_(t,h).k_j - lse[s][t][h])
 // over the (t, j) pairs that tree_attention attends, with its q, mask, scale and lse. mass fp32
-// [n_seqs][n_kv_heads][max_ctx]; node_weight fp32 [n_seqs][n_nodes], NULL for all ones. Nodes of
-// weight 0 (rejected drafts) are left out altogether, and rows with lse = -inf add nothing. Every
+// [n_seqs][n_kv_heads][max_ctx]; node_weight fp32 [n_seqs][n_nodes], NULL for all ones. Only nodes of
+// weight > 0 count: rejected drafts (weight 0, or any other) are left out altogether, whatever
+// their q and lse hold, and rows with lse = -inf add nothing. Every
 // value has one owner, which adds in a fixed order: equal inputs give equal bits.
 jinf_status jinf_b200_attention_mass(float* mass, const void* q, int64_t q_seq_stride, int64_t q_node_stride,
                                      int n_heads, int n_nodes, const jinf_b200_kv* kv, const int32_t* n_past,

@@ -24,7 +24,7 @@ struct MassSmem {
     uint8_t q[2][MROWS * HD * 2];
     float bias[2][MROWS];    // -lse log2 e
     float weight[2][MROWS];
-    int node[JINF_TREE_MAX_NODES];  // nodes of weight != 0, ascending
+    int node[JINF_TREE_MAX_NODES];  // nodes of weight > 0, ascending
     int n_nodes;
 };
 
@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(MW * 32)
         int n = 0;
         for (int t0 = 0; t0 < p.n_nodes; t0 += 32) {
             const int t = t0 + lane;
-            const bool on = t < p.n_nodes && (!weight || weight[(size_t)seq * p.n_nodes + t] != 0.f);
+            const bool on = t < p.n_nodes && (!weight || weight[(size_t)seq * p.n_nodes + t] > 0.f);
             const uint32_t b = __ballot_sync(JINF_FULL_MASK, on);
             if (on) sm.node[n + __popc(b & ((1u << lane) - 1u))] = t;
             n += __popc(b);

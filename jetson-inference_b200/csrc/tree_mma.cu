@@ -118,21 +118,7 @@ __global__ void __launch_bounds__(XT, 1)
     // barrier must know that x - 1 is over and that x + 1 is not. So each role waits for every
     // phase of a barrier in order (or for one whose predecessor an earlier wait implies), and no phase
     // ends twice before it has looked.
-    // a bounded wait that also ends when another role gave up
-    auto wait = [&](uint64_t& bar, uint32_t parity) -> bool {
-        const uint32_t b = su32(&bar);
-        for (unsigned long long it = 0; it < MB_SPIN; ++it) {
-            if (mb_try(b, parity)) return true;
-            if ((it & 255) == 255 && *(volatile int*)&ms.abort) return false;
-        }
-        atomicExch(&ms.abort, 1);
-        atomicExch(p.err, 1);
-        return false;
-    };
-    // the same for a whole warp, which stays converged
-    auto wait_all = [&](uint64_t& bar, uint32_t parity) -> bool {
-        return __all_sync(JINF_FULL_MASK, wait(bar, parity));
-    };
+    auto wait_all = [&](uint64_t& bar, uint32_t parity) { return mb_wait_warp(su32(&bar), parity, &ms.abort, p.err); };
     // One arrival per warp, after what all its lanes did: 128 of them on one mbarrier would take about
     // 1200 cycles.
     auto arrive_warp = [&](uint64_t& bar) {
@@ -147,38 +133,43 @@ __global__ void __launch_bounds__(XT, 1)
     auto tile_at = [](int x, int n) { return x == 2 * n - 1 ? n - 1 : x & 1 ? (x + 1) / 2 : x ? x / 2 - 1 : 0; };
 
     if (warp == 0) {
-        if (lane == 0) {  // ---- copies
-            uint32_t pos = 0, units = 0;
-            bool ok = true;
-            while (ok && share.next(p, sg)) {
-                const int n = sg.t1 - sg.t0;
-                // Q: the rows of tile_nodes nodes, node by node, are one box; nodes past the last are zeros
-                if (units && !(ok = wait(ms.q_free, (units - 1) & 1))) break;
-                const uint32_t qbar = su32(&ms.q_full);
-                mb_expect(qbar, (two ? 2 : 1) * (HD / 64) * 128 * tile_rows);
+        // ---- copies
+        uint32_t pos = 0, units = 0;
+        bool ok = true;
+        while (ok && share.next(p, sg)) {
+            const int n = sg.t1 - sg.t0;
+            // Q: the rows of tile_nodes nodes, node by node, are one box; nodes past the last are zeros
+            if (units && !(ok = wait_all(ms.q_free, (units - 1) & 1))) break;
+            if (lane == 0) {
+                const uint32_t bar = su32(&ms.q_full);
+                mb_expect(bar, (two ? 2 : 1) * (HD / 64) * 128 * tile_rows);
                 for (int w = 0; w < (two ? 2 : 1); ++w)
 #pragma unroll
                     for (int a = 0; a < HD / 64; ++a)
                         tma_load_4d(s_q + w * TILE + a * ATOM, &tmq, 64 * a, sg.head * p.group,
-                                    row0 / p.group + w * p.tile_nodes, sg.seq, qbar);
-                ++units;
-                for (int x = 0; ok && x < 2 * n; ++x, ++pos) {
-                    const bool is_k = k_at(x, n);
-                    const int i = tile_at(x, n);
-                    const uint32_t slot = pos % ST, fill = pos / ST;
-                    if (fill && !(ok = wait(ms.empty[slot], (fill - 1) & 1))) break;
+                                    row0 / p.group + w * p.tile_nodes, sg.seq, bar);
+            }
+            __syncwarp();
+            ++units;
+            for (int x = 0; x < 2 * n; ++x, ++pos) {
+                const bool is_k = k_at(x, n);
+                const int i = tile_at(x, n);
+                const uint32_t slot = pos % ST, fill = pos / ST;
+                if (fill && !(ok = wait_all(ms.empty[slot], (fill - 1) & 1))) break;
+                if (lane == 0) {
                     const uint32_t bar = su32(&ms.full[slot]);
                     mb_expect(bar, TILE);
 #pragma unroll
                     for (int a = 0; a < HD / 64; ++a)
-                        tma_load_4d(s_kv + slot * TILE + a * ATOM, is_k ? &tmk : &tmv, 64 * a, (sg.t0 + i) * KV_TILE,
-                                    sg.head, sg.seq, bar);
+                        tma_load_4d(s_kv + slot * TILE + a * ATOM, is_k ? &tmk : &tmv, 64 * a, (sg.t0 + i) * KV_TILE, sg.head,
+                                    sg.seq, bar);
                 }
+                __syncwarp();
             }
-            if (!ok) {  // leave no copy in flight
-                if (units) mb_wait(su32(&ms.q_full), (units - 1) & 1);
-                for (uint32_t s = 0; s < ST && s < pos; ++s) mb_wait(su32(&ms.full[s]), ((pos - 1 - s) / ST) & 1);
-            }
+        }
+        if (!ok && lane == 0) {  // leave no copy in flight
+            if (units) mb_wait(su32(&ms.q_full), (units - 1) & 1);
+            for (uint32_t s = 0; s < ST && s < pos; ++s) mb_wait(su32(&ms.full[s]), ((pos - 1 - s) / ST) & 1);
         }
     } else if (warp == 1 || warp == 3) {
         // ---- MMAs of group w, one lane issuing for the converged warp

@@ -47,6 +47,26 @@ __device__ __forceinline__ bool elect_one() {
     return e;
 }
 
+// The polling part of wait_warp: not inlined, so that a wait whose phase is already over, the usual
+// case in a pipeline that keeps up, is a dozen instructions at each of its many places.
+__device__ __noinline__ static bool mb_poll_warp(uint32_t b, uint32_t parity, int* abort_flag, int* err) {
+    bool done = false;
+    for (unsigned long long it = 0; it < MB_SPIN && !done; ++it) {
+        done = __all_sync(0xffffffffu, mb_try(b, parity));
+        if ((it & 255) == 255 && __any_sync(0xffffffffu, *(volatile int*)abort_flag)) break;
+    }
+    if (!done) {
+        atomicExch(abort_flag, 1);
+        atomicExch(err, 1);
+    }
+    return done;
+}
+// Bounded wait of a converged warp for phase `parity` of the mbarrier; false when it ran out or another
+// warp of the CTA gave up (`abort_flag`, shared memory), and then *err is set.
+__device__ __forceinline__ bool mb_wait_warp(uint32_t b, uint32_t parity, int* abort_flag, int* err) {
+    return __all_sync(0xffffffffu, mb_try(b, parity)) || mb_poll_warp(b, parity, abort_flag, err);
+}
+
 // raw bytes global -> shared on an mbarrier (16-byte aligned, a multiple of 16 bytes)
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
