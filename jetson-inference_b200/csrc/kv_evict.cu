@@ -10,6 +10,17 @@
 namespace jinf {
 namespace {
 
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// *p of CTA `rank` of the cluster (p: this CTA's own)
+__device__ __forceinline__ uint32_t remote_u32(const uint32_t* p, int rank) {
+    uint32_t a, v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
 // Order of the masses as unsigned words: larger mass, larger word; NaN below everything; -0 as 0.
 __device__ __forceinline__ uint32_t mass_rank(float x) {
     if (isnan(x)) return 0u;
@@ -17,99 +28,150 @@ __device__ __forceinline__ uint32_t mass_rank(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-constexpr int SEL_THREADS = 1024;
+constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2 * SEL_THREADS;
+constexpr int SEL_KEYS = 40960;  // ranks of a CTA's slice kept in shared memory; a longer slice is read again each pass
 
-// k_evict_select: the kept row numbers of one (sequence, kv head) per CTA. The n_pick rows of
-// largest mass among rows n_sink .. n - n_recent - 1 by radix selection, 8 bits of the rank at
-// a time (the count of ranks above a prefix), then the ids in order by a block scan.
+// k_evict_select: the kept row numbers of one (sequence, kv head) per cluster of C CTAs, a contiguous
+// slice of the rows each. The n_pick rows of largest mass among rows n_sink .. n - n_recent - 1 by
+// radix selection, 11, 11 and 10 bits of the rank: the slices' counts are added over distributed
+// shared memory, one cluster barrier a round. Then every warp counts what it keeps of its own rows, a
+// scan over warps and CTAs gives the places, and the warps write the numbers in order.
+// Latency bounds it: the masses of 8192 rows are 32 KB. Clusters pay from about 16384 rows on (below
+// that their barriers cost more than one CTA's passes).
+template <int C>
 __global__ void __launch_bounds__(SEL_THREADS)
     k_evict_select(const float* __restrict__ mass, const int32_t* __restrict__ n_rows, int32_t* __restrict__ ids,
-                   int32_t* __restrict__ n_out, int n_kv_heads, int max_ctx, int n_keep, int n_sink, int n_recent) {
-    __shared__ int hist[256];
-    __shared__ int wsum[32];
-    __shared__ int pick_digit, pick_left;
-    const int seq = blockIdx.x / n_kv_heads, head = blockIdx.x % n_kv_heads, tid = threadIdx.x;
+                   int32_t* __restrict__ n_out, int n_kv_heads, int max_ctx, int n_keep, int n_sink, int n_recent, int n_keys) {
+    extern __shared__ uint32_t keys[];  // n_keys of them
+    __shared__ uint32_t hist[2][SEL_BINS];
+    __shared__ uint32_t wsum[SEL_WARPS];
+    __shared__ uint32_t pick[2];                 // digit, left
+    __shared__ int wsure[SEL_WARPS], wequal[SEL_WARPS];
+    __shared__ int total[2];                     // of this CTA: rows kept for sure, rows of the last rank
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int unit = blockIdx.x / C, part = blockIdx.x % C;
+    const int seq = unit / n_kv_heads, head = unit % n_kv_heads;
     const int n = min(max(n_rows[seq], 0), max_ctx);
-    const float* mp = mass + (size_t)blockIdx.x * max_ctx;
-    int32_t* op = ids + (size_t)blockIdx.x * n_keep;
+    const float* mp = mass + (size_t)unit * max_ctx;
+    int32_t* op = ids + (size_t)unit * n_keep;
+    pdl_trigger();  // the moves' CTAs may be set up; they wait for this kernel's end
     const int kept = min(n, n_keep);
-    if (n_out && head == 0 && tid == 0) n_out[seq] = kept;
-    for (int i = kept + tid; i < n_keep; i += SEL_THREADS) op[i] = -1;
-    if (n <= n_keep) {
-        for (int i = tid; i < n; i += SEL_THREADS) op[i] = i;
+    if (n_out && head == 0 && part == 0 && tid == 0) n_out[seq] = kept;
+    for (int i = kept + part * SEL_THREADS + tid; i < n_keep; i += C * SEL_THREADS) op[i] = -1;
+    if (n <= n_keep) {  // the same in the whole cluster
+        for (int i = part * SEL_THREADS + tid; i < n; i += C * SEL_THREADS) op[i] = i;
         return;
     }
     const int lo = n_sink, hi = n - n_recent;  // hi - lo > n_keep - n_sink - n_recent >= 0
-    int left = n_keep - n_sink - n_recent;     // still to be picked among the ranks that match the prefix
+    // rows of this CTA: whole warps' spans, so that a warp's rows are consecutive
+    const int span = (n + C * SEL_THREADS - 1) / (C * SEL_THREADS) * 32;  // rows of a warp
+    const int base = part * SEL_WARPS * span, limit = min(n, base + SEL_WARPS * span);
+    const bool stage = SEL_WARPS * span <= n_keys;
+    if (stage)
+        for (int i = base + tid; i < limit; i += SEL_THREADS) keys[i - base] = mass_rank(mp[i]);
+    auto rank_of = [&](int i) { return stage ? keys[i - base] : mass_rank(mp[i]); };
+
+    uint32_t left = n_keep - n_sink - n_recent;  // still to be picked among the ranks that match the prefix
+    const bool none = left == 0;
     uint32_t prefix = 0, mask = 0;
-    if (left > 0) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            for (int i = lo + tid; i < hi; i += SEL_THREADS) {
-                const uint32_t r = mass_rank(mp[i]);
-                if ((r & mask) == prefix) atomicAdd(&hist[(r >> shift) & 255], 1);
-            }
-            __syncthreads();
-            if (tid == 0) {  // the digit whose bin holds the left-th largest
-                int d = 255, above = 0;
-                while (d > 0 && above + hist[d] < left) above += hist[d--];
-                pick_digit = d;
-                pick_left = left - above;
-            }
-            __syncthreads();
-            prefix |= (uint32_t)pick_digit << shift;
-            mask |= 255u << shift;
-            left = pick_left;
-            __syncthreads();
+    for (int round = 0; round < 3 && !none; ++round) {
+        const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
+        const uint32_t digit = round == 2 ? 1023u : 2047u;
+        uint32_t* h = hist[round & 1];
+        h[tid] = 0;
+        h[tid + SEL_THREADS] = 0;
+        __syncthreads();
+        for (int i = max(lo, base) + tid; i < min(hi, limit); i += SEL_THREADS) {
+            const uint32_t r = rank_of(i);
+            if ((r & mask) == prefix) atomicAdd(&h[(r >> shift) & digit], 1u);
         }
+        if constexpr (C > 1) cluster_barrier(); else __syncthreads();
+        // bins SEL_BINS - 1 - 2 tid and the one below: how many have a larger digit, and these
+        const int bin = SEL_BINS - 1 - 2 * tid;
+        uint32_t a = 0, b = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            a += C > 1 ? remote_u32(&h[bin], c) : h[bin];
+            b += C > 1 ? remote_u32(&h[bin - 1], c) : h[bin - 1];
+        }
+        uint32_t upto = a + b;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(JINF_FULL_MASK, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) wsum[warp] = upto;
+        __syncthreads();
+        upto += __reduce_add_sync(JINF_FULL_MASK, lane < warp ? wsum[lane] : 0u);
+        const uint32_t above = upto - a - b;
+        if (upto >= left && above < left) {  // one of the two bins holds the left-th largest
+            const bool first = above + a >= left;
+            pick[0] = first ? bin : bin - 1;
+            pick[1] = first ? left - above : left - above - a;
+        }
+        __syncthreads();
+        prefix |= pick[0] << shift;
+        mask |= digit << shift;
+        left = pick[1];
     }
     // ranks above `prefix` stay; of those equal to it the first `left`
-    const bool none = n_keep == n_sink + n_recent;
-    int kept_before = 0, equal_before = 0;
-    for (int i0 = 0; i0 < n; i0 += SEL_THREADS) {
-        const int i = i0 + tid;
-        bool keep = false, equal = false;
-        if (i < n) {
-            if (i < lo || i >= hi) keep = true;
-            else if (!none) {
-                const uint32_t r = mass_rank(mp[i]);
-                keep = r > prefix;
-                equal = r == prefix;
-            }
-        }
-        for (int pass = 0; pass < 2; ++pass) {  // the equal ones' places first, then the kept ones'
-            const bool f = pass ? keep : equal;
-            const uint32_t b = __ballot_sync(JINF_FULL_MASK, f);
-            if ((tid & 31) == 0) wsum[tid >> 5] = __popc(b);
-            __syncthreads();
-            int before = __popc(b & ((1u << (tid & 31)) - 1u)), all = 0;
-            for (int w = 0; w < 32; ++w) {
-                if (w < (tid >> 5)) before += wsum[w];
-                all += wsum[w];
-            }
-            __syncthreads();
-            if (!pass) {
-                if (equal && equal_before + before < left) keep = true;
-                equal_before += all;
-            } else {
-                if (keep) op[kept_before + before] = i;
-                kept_before += all;
-            }
-        }
+    auto sure = [&](int i) { return i < limit && (i < lo || i >= hi || (!none && rank_of(i) > prefix)); };
+    auto equal = [&](int i) { return i < limit && i >= lo && i < hi && !none && rank_of(i) == prefix; };
+    __syncthreads();  // the staged ranks, where no round ran
+    const int first = base + warp * span;
+    int n_sure = 0, n_equal = 0;
+    for (int i = first; i < first + span; i += 32) {
+        n_sure += __popc(__ballot_sync(JINF_FULL_MASK, sure(i + lane)));
+        n_equal += __popc(__ballot_sync(JINF_FULL_MASK, equal(i + lane)));
     }
+    if (lane == 0) {
+        wsure[warp] = n_sure;
+        wequal[warp] = n_equal;
+    }
+    __syncthreads();
+    // this warp's place: what the CTAs and warps before it keep
+    int place = 0, taken = 0;  // kept rows, and rows of the last rank, before
+    auto add = [&](int s, int e) {
+        place += s + min(max((int)left - taken, 0), e);
+        taken += e;
+    };
+    if constexpr (C > 1) {
+        if (warp == 0) {
+            const int s = (int)__reduce_add_sync(JINF_FULL_MASK, (unsigned)wsure[lane]);
+            const int e = (int)__reduce_add_sync(JINF_FULL_MASK, (unsigned)wequal[lane]);
+            if (lane == 0) {
+                total[0] = s;
+                total[1] = e;
+            }
+        }
+        cluster_barrier();
+        for (int c = 0; c < part; ++c)
+            add((int)remote_u32((uint32_t*)&total[0], c), (int)remote_u32((uint32_t*)&total[1], c));
+    }
+    for (int w = 0; w < warp; ++w) add(wsure[w], wequal[w]);
+    for (int i = first; i < first + span; i += 32) {
+        const bool eq = equal(i + lane);
+        const uint32_t before = (1u << lane) - 1u, be = __ballot_sync(JINF_FULL_MASK, eq);
+        const bool keep = sure(i + lane) || (eq && taken + __popc(be & before) < (int)left);
+        const uint32_t bk = __ballot_sync(JINF_FULL_MASK, keep);
+        if (keep) op[place + __popc(bk & before)] = i + lane;
+        place += __popc(bk);
+        taken += __popc(be);
+    }
+    if constexpr (C > 1) cluster_barrier();  // no CTA leaves while another may read its counts
 }
 
-constexpr int MV_THREADS = 256, MV_CHUNKS = 4, MV_BATCH = 4;
+constexpr int MV_THREADS = 256, MV_CHUNKS = 4, MV_BATCH = 8;
 constexpr int MV_ROWS = MV_THREADS / MV_CHUNKS * MV_BATCH;  // rows of a batch
 
-// k_evict_move: row ids[i] -> row i. blockIdx.x = (sequence, kv head); blockIdx.y = K or V and a
-// 64-byte column of the rows, and the mass (one more); blockIdx.z = batches (one block in place).
-// Source and destination may be the same memory: no pointer to either is __restrict__.
+// k_evict_move, in place: row ids[i] -> row i. blockIdx.x = (sequence, kv head); blockIdx.y = K or V and
+// a 64-byte column of the rows, and the mass (one more). A block takes the batches of rows in order.
+// Source and destination are the same memory: no pointer to either is __restrict__.
 __global__ void __launch_bounds__(MV_THREADS)
     k_evict_move(const KvPlanes src, const KvPlanes dst, const float* mass, float* mass_out,
                  const int32_t* __restrict__ ids, const int32_t* __restrict__ n_rows, int n_kv_heads, int row_bytes,
                  int n_keep) {
+    pdl_wait();
     const int seq = blockIdx.x / n_kv_heads, head = blockIdx.x % n_kv_heads, tid = threadIdx.x;
     const int n = min(min(max(n_rows[seq], 0), src.max_ctx), n_keep);
     const int32_t* ip = ids + (size_t)blockIdx.x * n_keep;
@@ -117,7 +179,7 @@ __global__ void __launch_bounds__(MV_THREADS)
     if ((int)blockIdx.y == 2 * cols) {
         const float* from = mass + (size_t)blockIdx.x * src.max_ctx;
         float* to = mass_out + (size_t)blockIdx.x * dst.max_ctx;
-        for (int i0 = blockIdx.z * MV_THREADS; i0 < n; i0 += gridDim.z * MV_THREADS) {
+        for (int i0 = 0; i0 < n; i0 += MV_THREADS) {
             const int i = i0 + tid;
             float x = 0.f;
             if (i < n) x = from[ip[i]];
@@ -131,7 +193,7 @@ __global__ void __launch_bounds__(MV_THREADS)
     const int64_t col = (blockIdx.y % cols) * 64 + (tid % MV_CHUNKS) * 16;
     const uint8_t* from = (is_v ? src.v : src.k) + seq * src.seq + head * src.head + col;
     uint8_t* to = (is_v ? dst.v : dst.k) + seq * dst.seq + head * dst.head + col;
-    for (int b0 = blockIdx.z * MV_ROWS; b0 < n; b0 += gridDim.z * MV_ROWS) {
+    for (int b0 = 0; b0 < n; b0 += MV_ROWS) {
         uint4 x[MV_BATCH];
 #pragma unroll
         for (int j = 0; j < MV_BATCH; ++j) {
@@ -145,6 +207,48 @@ __global__ void __launch_bounds__(MV_THREADS)
             if (i < n) *reinterpret_cast<uint4*>(to + (int64_t)i * dst.row) = x[j];
         }
         __syncthreads();
+    }
+}
+
+constexpr int CP_BATCH = 4;
+
+// k_evict_copy, into another cache: whole rows (CH 16-byte chunks), CP_BATCH of them per thread in
+// flight. blockIdx.x = batch of rows, so that neighbouring blocks read neighbouring rows; blockIdx.y =
+// (sequence, kv head). HBM bounds it: 256 heads from 32768 rows to 8192 in 0.33 ms, 6.5 TB/s (8 rows a
+// thread 0.43 ms, heads before batches in the grid 0.34).
+template <int CH>
+__global__ void __launch_bounds__(MV_THREADS)
+    k_evict_copy(const KvPlanes src, const KvPlanes dst, const float* __restrict__ mass, float* __restrict__ mass_out,
+                 const int32_t* __restrict__ ids, const int32_t* __restrict__ n_rows, int n_units, int n_kv_heads, int n_keep) {
+    constexpr int LANES = MV_THREADS / CH;  // rows side by side
+    pdl_wait();
+    const int c = threadIdx.x % CH, i0 = blockIdx.x * LANES * CP_BATCH + threadIdx.x / CH;
+    for (int unit = blockIdx.y; unit < n_units; unit += gridDim.y) {
+        const int seq = unit / n_kv_heads, head = unit % n_kv_heads;
+        const int n = min(min(max(n_rows[seq], 0), src.max_ctx), n_keep);
+        const int32_t* ip = ids + (size_t)unit * n_keep;
+        const int64_t so = seq * src.seq + head * src.head + c * 16, dof = seq * dst.seq + head * dst.head + c * 16;
+        int from[CP_BATCH];
+#pragma unroll
+        for (int j = 0; j < CP_BATCH; ++j) from[j] = i0 + j * LANES < n ? __ldg(ip + i0 + j * LANES) : -1;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            const uint8_t* s = (v ? src.v : src.k) + so;
+            uint8_t* d = (v ? dst.v : dst.k) + dof;
+            uint4 x[CP_BATCH];
+#pragma unroll
+            for (int j = 0; j < CP_BATCH; ++j)
+                if (from[j] >= 0) x[j] = __ldcs(reinterpret_cast<const uint4*>(s + from[j] * src.row));
+#pragma unroll
+            for (int j = 0; j < CP_BATCH; ++j)
+                if (from[j] >= 0) __stcs(reinterpret_cast<uint4*>(d + (i0 + j * LANES) * dst.row), x[j]);
+        }
+        if (mass_out && c == 0) {
+#pragma unroll
+            for (int j = 0; j < CP_BATCH; ++j)
+                if (from[j] >= 0)
+                    mass_out[(size_t)unit * dst.max_ctx + i0 + j * LANES] = __ldg(mass + (size_t)unit * src.max_ctx + from[j]);
+        }
     }
 }
 
@@ -196,21 +300,57 @@ __global__ void __launch_bounds__(CM_WARPS * 32)
     if (n_out && head == 0 && lane == 0) n_out[seq] = past + n;
 }
 
+template <int C>
+cudaError_t launch_select(int units, const float* mass, const int32_t* n_rows, int32_t* ids, int32_t* n_out, int n_kv_heads,
+                          int max_ctx, int n_keep, int n_sink, int n_recent, cudaStream_t s) {
+    const int slice = (max_ctx + C * SEL_THREADS - 1) / (C * SEL_THREADS) * SEL_THREADS;
+    const int n_keys = slice <= SEL_KEYS ? slice : 0;
+    const cudaError_t e =
+        cudaFuncSetAttribute(k_evict_select<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_KEYS * (int)sizeof(uint32_t));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * C));
+    cfg.blockDim = dim3(SEL_THREADS);
+    cfg.dynamicSmemBytes = sizeof(uint32_t) * (size_t)n_keys;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = C > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, k_evict_select<C>, mass, n_rows, ids, n_out, n_kv_heads, max_ctx, n_keep, n_sink, n_recent, n_keys);
+}
+
 }  // namespace
 
 cudaError_t kv_evict_launch(const KvPlanes& src, const KvPlanes& dst, bool in_place, const float* mass, float* mass_out,
                             const int32_t* n_rows, int32_t* ids, int32_t* n_out, int n_seqs, int n_kv_heads,
                             int row_bytes, int n_keep, int n_sink, int n_recent, cudaStream_t s) {
     const int units = n_seqs * n_kv_heads;
-    k_evict_select<<<units, SEL_THREADS, 0, s>>>(mass, n_rows, ids, n_out, n_kv_heads, src.max_ctx, n_keep, n_sink,
-                                                 n_recent);
-    cudaError_t e = cudaGetLastError();
+    // One CTA per head up to 16384 rows, or where the heads fill the SMs and their ranks shared memory
+    // (256 heads of 32768 rows: see below); else clusters of 8.
+    cudaError_t e = src.max_ctx <= 16384 || (src.max_ctx <= SEL_KEYS && units >= kv_device_sms())
+                        ? launch_select<1>(units, mass, n_rows, ids, n_out, n_kv_heads, src.max_ctx, n_keep, n_sink, n_recent, s)
+                        : launch_select<8>(units, mass, n_rows, ids, n_out, n_kv_heads, src.max_ctx, n_keep, n_sink, n_recent, s);
     if (e != cudaSuccess) return e;
-    const int batches = (n_keep + MV_ROWS - 1) / MV_ROWS;
-    const dim3 grid((unsigned)units, (unsigned)(2 * (row_bytes / 64) + (mass_out ? 1 : 0)),
-                    (unsigned)(in_place ? 1 : (batches < 64 ? batches : 64)));
-    k_evict_move<<<grid, MV_THREADS, 0, s>>>(src, dst, mass, mass_out, ids, n_rows, n_kv_heads, row_bytes, n_keep);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(MV_THREADS);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (in_place) {
+        cfg.gridDim = dim3((unsigned)units, (unsigned)(2 * (row_bytes / 64) + (mass_out ? 1 : 0)));
+        return cudaLaunchKernelEx(&cfg, k_evict_move, src, dst, mass, mass_out, ids, n_rows, n_kv_heads, row_bytes, n_keep);
+    }
+    const int ch = row_bytes / 16, rows = MV_THREADS / ch * CP_BATCH, batches = (n_keep + rows - 1) / rows;
+    cfg.gridDim = dim3((unsigned)batches, (unsigned)(units < 65535 ? units : 65535));
+    return ch == 8 ? cudaLaunchKernelEx(&cfg, k_evict_copy<8>, src, dst, mass, mass_out, (const int32_t*)ids, n_rows, units, n_kv_heads, n_keep)
+                   : cudaLaunchKernelEx(&cfg, k_evict_copy<16>, src, dst, mass, mass_out, (const int32_t*)ids, n_rows, units, n_kv_heads, n_keep);
 }
 
 cudaError_t tree_commit_launch(const KvPlanes& kv, float* mass, const int32_t* n_past, int max_past,

@@ -290,6 +290,8 @@ EVICT = [  # (dtype, hd, kv heads, lengths, ctx, keep, sink, recent)
     (F16, 128, 8, [2048], 2048, 1, 0, 0),
     (F16, 128, 2, [40000], 40000, 3001, 4, 256),
     (F16, 64, 1, [140001], 140001, 1025, 0, 1),
+    (F16, 64, 1, [400000, 1000, 70000], 400000, 990, 3, 5),  # slices too long for shared memory, and short ones
+    (BF16, 64, 3, [16384, 16385, 1], 16385, 4000, 100, 0),
 ]
 
 
