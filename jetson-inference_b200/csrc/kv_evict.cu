@@ -305,8 +305,7 @@ cudaError_t launch_select(int units, const float* mass, const int32_t* n_rows, i
                           int max_ctx, int n_keep, int n_sink, int n_recent, cudaStream_t s) {
     const int slice = (max_ctx + C * SEL_THREADS - 1) / (C * SEL_THREADS) * SEL_THREADS;
     const int n_keys = slice <= SEL_KEYS ? slice : 0;
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_evict_select<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_KEYS * (int)sizeof(uint32_t));
+    const cudaError_t e = kv_allow_smem<k_evict_select<C>>(SEL_KEYS * (int)sizeof(uint32_t));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * C));

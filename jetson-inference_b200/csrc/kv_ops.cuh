@@ -9,6 +9,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 namespace jinf {
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -232,6 +234,18 @@ __device__ __forceinline__ int shared_units(const TreeParams& p, int g, const Sh
 }
 
 int kv_device_sms();  // SMs of the current device (cached per device)
+
+// Lets `kernel` have `smem` bytes of dynamic shared memory, set once per kernel and device.
+template <auto kernel>
+inline cudaError_t kv_allow_smem(int smem) {
+    static std::atomic<uint64_t> done;  // a bit per device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev) & 1)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return e;
+}
 
 // Key tiles of K or V, [seq][head][row][hd], as boxes of 64 columns x KV_TILE rows
 inline bool kv_tile_map(CUtensorMap* map, const void* base, const TreeParams& p, bool bf, int hd) {

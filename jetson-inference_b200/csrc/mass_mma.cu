@@ -455,7 +455,7 @@ cudaError_t launch_mass_mma(const TreeParams& p, const float* lse, const float* 
     if (!kv_tile_map(&mk, p.k, p, BF, HD) ||
         !rows_map(&mq, p.q, BF, HD, p.n_heads, HD, p.n_nodes, p.q_node, p.n_seqs, p.q_seq, p.group, p.tile_nodes))
         return cudaErrorInvalidValue;
-    const cudaError_t e = cudaFuncSetAttribute(k_mass_mma<BF, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassMma<HD>::TOTAL);
+    const cudaError_t e = kv_allow_smem<k_mass_mma<BF, HD>>(MassMma<HD>::TOTAL);
     if (e != cudaSuccess) return e;
     const int64_t tiles = (int64_t)p.n_seqs * p.n_kv_heads * ((p.max_past + p.n_nodes + KV_TILE - 1) / KV_TILE);
     const int sms = kv_device_sms();

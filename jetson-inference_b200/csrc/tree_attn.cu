@@ -326,8 +326,8 @@ template <bool BF, int HD>
 cudaError_t launch_rows(const TreeParams& p, const TreePlan& plan, uint16_t* out, float* lse, void* ws, cudaStream_t s) {
     const int grid = plan.n_groups * plan.row_blocks;
     return plan.block_rows <= 16
-               ? launch_coop(k_tree_rows<BF, HD, 1>, grid, TW * 32, RowsSmem<HD, 1>::TOTAL, s, p, out, lse, ws)
-               : launch_coop(k_tree_rows<BF, HD, 2>, grid, TW * 32, RowsSmem<HD, 2>::TOTAL, s, p, out, lse, ws);
+               ? launch_coop<k_tree_rows<BF, HD, 1>>(grid, TW * 32, RowsSmem<HD, 1>::TOTAL, s, p, out, lse, ws)
+               : launch_coop<k_tree_rows<BF, HD, 2>>(grid, TW * 32, RowsSmem<HD, 2>::TOTAL, s, p, out, lse, ws);
 }
 
 }  // namespace

@@ -543,8 +543,7 @@ cudaError_t launch_mma(const TreeParams& p, const TreePlan& plan, uint16_t* out,
     if (!rows_map(&mq, p.q, BF, HD, p.n_heads, HD, p.n_nodes, p.q_node, p.n_seqs, p.q_seq, p.group, p.tile_nodes) ||
         !kv_tile_map(&mk, p.k, p, BF, HD) || !kv_tile_map(&mv, p.v, p, BF, HD))
         return cudaErrorInvalidValue;
-    return launch_coop(k_tree_mma<BF, HD>, plan.n_groups * plan.row_blocks, XT, MmaSmem<HD>::TOTAL, s, mq, mk, mv, p, out, lse,
-                       ws);
+    return launch_coop<k_tree_mma<BF, HD>>(plan.n_groups * plan.row_blocks, XT, MmaSmem<HD>::TOTAL, s, mq, mk, mv, p, out, lse, ws);
 }
 
 }  // namespace

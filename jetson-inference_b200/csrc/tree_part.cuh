@@ -130,14 +130,14 @@ __device__ __forceinline__ void join_units(const TreeParams& p, JoinPlan& plan, 
     }
 }
 
-template <typename K, typename... A>
-cudaError_t launch_coop(K kernel, int grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <auto kernel, typename... A>
+cudaError_t launch_coop(int grid, int threads, int smem, cudaStream_t s, const A&... args) {
+    const cudaError_t e = kv_allow_smem<kernel>(smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeCooperative;

@@ -189,10 +189,18 @@ class KvView:
         self.struct = L.KvStruct(k.data_ptr(), v.data_ptr(), L.F16 if k.dtype == torch.float16 else L.BF16, *k.shape[:2],
                                  self.head_dim, self.max_ctx, *k.stride()[:3])
         self.ref = C.addressof(self.struct)
+        # what every call needs, looked up once
+        self._int, self._float, self._index = torch.int32, torch.float32, k.device.index
+        self._per_seq, self._per_row = (self.n_seqs,), (self.n_seqs, self.n_kv_heads, self.max_ctx)
+        self._raw_stream = torch._C._cuda_getCurrentRawStream
+        self._ws = {}
+
+    def _stream(self, stream):
+        return stream.cuda_stream if stream is not None else self._raw_stream(self._index)
 
 
 def _dense(t, name: str, dtype, shape) -> int:
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or not t.is_cuda:
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or not t.is_cuda:
         raise ValueError(f"{name}: a contiguous CUDA tensor {tuple(shape)} of {dtype} is needed, got "
                          f"{tuple(t.shape)} of {t.dtype}")
     return t.data_ptr()
@@ -201,23 +209,23 @@ def _dense(t, name: str, dtype, shape) -> int:
 def _query(q, kv: KvView):
     if q.dim() == 3:
         q = q.unsqueeze(0)
-    if q.dim() != 4 or q.shape[0] != kv.n_seqs or q.shape[3] != kv.head_dim or q.dtype != kv.dtype or not q.is_cuda:
+    shape, st = q.shape, q.stride()
+    if len(shape) != 4 or shape[0] != kv.n_seqs or shape[3] != kv.head_dim or q.dtype != kv.dtype or not q.is_cuda:
         raise ValueError("q: a CUDA tensor [n_seqs, n_nodes, n_heads, head_dim] of the cache's type is needed")
-    st = q.stride()
     if st[3] != 1 or st[2] != kv.head_dim:
         raise ValueError("q: the heads of a node are consecutive, head_dim elements each")
-    return q, st
+    return q.data_ptr(), shape, st
 
 
 def _mask(mask, kv: KvView, nodes: int):
-    import torch
     if mask is None:
         return None, 0
-    words = (nodes + 31) // 32
-    if mask.dtype != torch.int32 or not mask.is_contiguous() or not mask.is_cuda or \
-            tuple(mask.shape) not in ((nodes, words), (kv.n_seqs, nodes, words)):
+    words, shape = (nodes + 31) // 32, mask.shape
+    per_seq = len(shape) == 3
+    if mask.dtype != kv._int or not mask.is_contiguous() or not mask.is_cuda or \
+            shape != ((kv.n_seqs, nodes, words) if per_seq else (nodes, words)):
         raise ValueError(f"mask: contiguous CUDA int32 words [{nodes}, {words}] (or one such mask per sequence)")
-    return mask.data_ptr(), nodes * words if mask.dim() == 3 else 0
+    return mask.data_ptr(), nodes * words if per_seq else 0
 
 
 def tree_mask(parents):
@@ -232,7 +240,10 @@ def tree_mask(parents):
 
 
 def tree_attention_workspace_bytes(kv: KvView, n_heads: int, n_nodes: int, max_past: int) -> int:
-    return int(L.lib.jinf_b200_tree_attention_workspace_bytes(kv.ref, n_heads, n_nodes, max_past))
+    key = (n_heads, n_nodes, max_past)
+    if key not in kv._ws:
+        kv._ws[key] = int(L.lib.jinf_b200_tree_attention_workspace_bytes(kv.ref, *key))
+    return kv._ws[key]
 
 
 def tree_attention(out, q, kv: KvView, n_past, max_past: int, workspace, mask=None, lse=None, scale=None,
@@ -240,42 +251,33 @@ def tree_attention(out, q, kv: KvView, n_past, max_past: int, workspace, mask=No
     """out [n_seqs, n_nodes, n_heads, head_dim]: attention of each sequence's new nodes over its n_past[s]
     cached rows and the tree rows behind them that `mask` lets each node see (None: causal). `workspace`:
     a zeroed uint8 tensor of tree_attention_workspace_bytes, kept from call to call."""
-    import torch
-    q, st = _query(q, kv)
-    _, nodes, nh, hd = q.shape
-    if out.dtype != kv.dtype or out.numel() != q.numel() or not out.is_contiguous() or not out.is_cuda:
-        raise ValueError("out: a contiguous CUDA tensor of q's shape and type is needed")
-    lse_p = None
-    if lse is not None:
-        if lse.dtype != torch.float32 or lse.numel() * hd != q.numel() or not lse.is_contiguous():
-            raise ValueError("lse: contiguous fp32 [n_seqs, n_nodes, n_heads]")
-        lse_p = lse.data_ptr()
-    if workspace.numel() * workspace.element_size() < tree_attention_workspace_bytes(kv, nh, nodes, max_past):
+    qp, shape, st = _query(q, kv)
+    nodes, nh, hd = shape[1], shape[2], shape[3]
+    op = _dense(out, "out", kv.dtype, shape if out.dim() == 4 else shape[1:])
+    lp = None if lse is None else _dense(lse, "lse", kv._float, shape[:3] if lse.dim() == 3 else shape[1:3])
+    if workspace.nbytes < tree_attention_workspace_bytes(kv, nh, nodes, max_past) or not workspace.is_cuda:
         raise ValueError("workspace is smaller than tree_attention_workspace_bytes")
     mp, ms = _mask(mask, kv, nodes)
-    L.check(L.lib.jinf_b200_tree_attention(out.data_ptr(), lse_p, q.data_ptr(), st[0], st[1], nh, nodes, kv.ref,
-                                           _dense(n_past, "n_past", torch.int32, (kv.n_seqs,)), max_past, mp, ms,
-                                           hd ** -0.5 if scale is None else scale, workspace.data_ptr(), _s(stream)),
-            "jinf_b200_tree_attention")
+    L.check(L.lib.jinf_b200_tree_attention(op, lp, qp, st[0], st[1], nh, nodes, kv.ref,
+                                           _dense(n_past, "n_past", kv._int, kv._per_seq), max_past, mp, ms,
+                                           hd ** -0.5 if scale is None else scale, workspace.data_ptr(),
+                                           kv._stream(stream)), "jinf_b200_tree_attention")
 
 
 def attention_mass(mass, q, kv: KvView, n_past, max_past: int, lse, mask=None, node_weight=None, scale=None,
                    stream=None) -> None:
-    """Adds to mass [n_seqs, n_kv_heads, max_ctx] the attention weight that the nodes (times node_weight
-    [n_seqs, n_nodes]; None: 1) gave each cached row, from tree_attention's q, mask and lse; the tree's own
-    rows are set, not added to."""
-    import torch
-    q, st = _query(q, kv)
-    _, nodes, nh, hd = q.shape
-    if lse.dtype != torch.float32 or lse.numel() * hd != q.numel() or not lse.is_contiguous() or not lse.is_cuda:
-        raise ValueError("lse: contiguous CUDA fp32 [n_seqs, n_nodes, n_heads]")
-    wp = None if node_weight is None else _dense(node_weight, "node_weight", torch.float32, (kv.n_seqs, nodes))
+    """Adds to mass [n_seqs, n_kv_heads, max_ctx] the attention weight that the nodes of positive node_weight
+    [n_seqs, n_nodes] (None: 1 each) gave each cached row, times that weight, from tree_attention's q, mask
+    and lse; the tree's own rows are set, not added to."""
+    qp, shape, st = _query(q, kv)
+    nodes, nh, hd = shape[1], shape[2], shape[3]
+    lp = _dense(lse, "lse", kv._float, shape[:3] if lse.dim() == 3 else shape[1:3])
+    wp = None if node_weight is None else _dense(node_weight, "node_weight", kv._float, shape[:2])
     mp, ms = _mask(mask, kv, nodes)
-    L.check(L.lib.jinf_b200_attention_mass(_dense(mass, "mass", torch.float32, (kv.n_seqs, kv.n_kv_heads, kv.max_ctx)),
-                                           q.data_ptr(), st[0], st[1], nh, nodes, kv.ref,
-                                           _dense(n_past, "n_past", torch.int32, (kv.n_seqs,)), max_past,
-                                           lse.data_ptr(), mp, ms, wp, hd ** -0.5 if scale is None else scale,
-                                           _s(stream)), "jinf_b200_attention_mass")
+    L.check(L.lib.jinf_b200_attention_mass(_dense(mass, "mass", kv._float, kv._per_row), qp, st[0], st[1], nh, nodes,
+                                           kv.ref, _dense(n_past, "n_past", kv._int, kv._per_seq), max_past, lp, mp, ms,
+                                           wp, hd ** -0.5 if scale is None else scale, kv._stream(stream)),
+            "jinf_b200_attention_mass")
 
 
 def kv_evict(kv: KvView, kv_out, mass, mass_out, n_rows, ids, n_out, n_keep: int, n_sink: int = 0, n_recent: int = 0,
@@ -283,32 +285,28 @@ def kv_evict(kv: KvView, kv_out, mass, mass_out, n_rows, ids, n_out, n_keep: int
     """Keeps n_keep rows per sequence and kv head: the first n_sink, the last n_recent and the heaviest
     others, in order, in kv_out / mass_out (None, or kv itself and mass: in place); ids
     [n_seqs, n_kv_heads, n_keep] and n_out [n_seqs] (may be None) receive the kept rows and their count."""
-    import torch
     out = kv if kv_out is None else kv_out
-    mo = None if mass_out is None else _dense(mass_out, "mass_out", torch.float32,
-                                              (kv.n_seqs, kv.n_kv_heads, out.max_ctx))
-    no = None if n_out is None else _dense(n_out, "n_out", torch.int32, (kv.n_seqs,))
-    L.check(L.lib.jinf_b200_kv_evict(kv.ref, out.ref,
-                                     _dense(mass, "mass", torch.float32, (kv.n_seqs, kv.n_kv_heads, kv.max_ctx)), mo,
-                                     _dense(n_rows, "n_rows", torch.int32, (kv.n_seqs,)),
-                                     _dense(ids, "ids", torch.int32, (kv.n_seqs, kv.n_kv_heads, n_keep)), no, n_keep,
-                                     n_sink, n_recent, _s(stream)), "jinf_b200_kv_evict")
+    mo = None if mass_out is None else _dense(mass_out, "mass_out", kv._float, out._per_row)
+    no = None if n_out is None else _dense(n_out, "n_out", kv._int, kv._per_seq)
+    L.check(L.lib.jinf_b200_kv_evict(kv.ref, out.ref, _dense(mass, "mass", kv._float, kv._per_row), mo,
+                                     _dense(n_rows, "n_rows", kv._int, kv._per_seq),
+                                     _dense(ids, "ids", kv._int, (kv.n_seqs, kv.n_kv_heads, n_keep)), no, n_keep,
+                                     n_sink, n_recent, kv._stream(stream)), "jinf_b200_kv_evict")
 
 
 def tree_commit(kv: KvView, mass, n_past, max_past: int, accepted, n_accepted, n_nodes: int, n_out=None,
                 stream=None) -> None:
     """Moves the rows of the accepted nodes (accepted [n_seqs, most], ascending, n_accepted[s] of them) up
     behind the cached rows, in place, with their mass (may be None); n_out[s] = n_past[s] + n_accepted[s]."""
-    import torch
-    mp = None if mass is None else _dense(mass, "mass", torch.float32, (kv.n_seqs, kv.n_kv_heads, kv.max_ctx))
-    no = None if n_out is None else _dense(n_out, "n_out", torch.int32, (kv.n_seqs,))
+    mp = None if mass is None else _dense(mass, "mass", kv._float, kv._per_row)
+    no = None if n_out is None else _dense(n_out, "n_out", kv._int, kv._per_seq)
     if accepted.dim() != 2:
         raise ValueError("accepted: int32 [n_seqs, most]")
-    L.check(L.lib.jinf_b200_tree_commit(kv.ref, mp, _dense(n_past, "n_past", torch.int32, (kv.n_seqs,)), max_past,
-                                        _dense(accepted, "accepted", torch.int32, (kv.n_seqs, accepted.shape[1])),
-                                        accepted.shape[1],
-                                        _dense(n_accepted, "n_accepted", torch.int32, (kv.n_seqs,)), n_nodes, no,
-                                        _s(stream)), "jinf_b200_tree_commit")
+    most = accepted.shape[1]
+    L.check(L.lib.jinf_b200_tree_commit(kv.ref, mp, _dense(n_past, "n_past", kv._int, kv._per_seq), max_past,
+                                        _dense(accepted, "accepted", kv._int, (kv.n_seqs, most)), most,
+                                        _dense(n_accepted, "n_accepted", kv._int, kv._per_seq), n_nodes, no,
+                                        kv._stream(stream)), "jinf_b200_tree_commit")
 
 
 def kv_ops_status() -> None:
