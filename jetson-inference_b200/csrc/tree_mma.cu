@@ -42,18 +42,18 @@ struct MmaSmem {
     static constexpr int OFF_MISC = OFF_KV + ST * TILE;
     struct Misc {
         uint64_t full[ST], empty[ST], vok[BAD_SETS];
-        uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2], flag_ok[2], drain[2], join, q_full, q_free;
+        uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2], flag_ok[2], drain[2], join, q_full[2], q_free, stagger;
         Share share;
         Shares all;
         JoinPlan plan;
         uint32_t tmem;
         int abort;
         uint32_t bad[BAD_SETS][4];
-        float jm[128], jl[128];
+        float jm[2][128], jl[2][128];
     };
-    static constexpr int TOTAL = OFF_MISC + (int)sizeof(Misc) + 1024;
+    static constexpr int TOTAL = OFF_MISC + (int)sizeof(Misc);  // from a 1024-byte boundary
 };
-static_assert(MmaSmem<128>::TOTAL + 256 <= 232448 && MmaSmem<64>::TOTAL + 256 <= 232448, "shared memory (with join_units')");
+static_assert(MmaSmem<128>::TOTAL <= 232448 && MmaSmem<64>::TOTAL <= 232448, "shared memory");
 
 template <bool BF, int HD>
 __global__ void __launch_bounds__(XT, 1)
@@ -63,8 +63,13 @@ __global__ void __launch_bounds__(XT, 1)
     using SM = MmaSmem<HD>;
     constexpr int TILE = SM::TILE, ST = SM::ST;
     constexpr uint32_t ID_QK = umma_idesc(BF, 128, 64, false), ID_PV = umma_idesc(BF, 128, HD, true);
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* sm = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    // The swizzled tiles need 1024-byte boundaries. The kernel has no other shared memory, so that this
+    // array starts on one; there is no room to round up, so a start elsewhere is an error.
+    extern __shared__ __align__(1024) uint8_t sm[];
+    if (su32(sm) & 1023) {
+        if (threadIdx.x == 0) atomicExch(p.err, 1);
+        return;
+    }
     typename SM::Misc& ms = *reinterpret_cast<typename SM::Misc*>(sm + SM::OFF_MISC);
     const uint32_t s_q = su32(sm), s_kv = s_q + SM::OFF_KV;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -90,8 +95,10 @@ __global__ void __launch_bounds__(XT, 1)
             mb_init(su32(&ms.drain[w]), 1);
         }
         mb_init(su32(&ms.join), 8);
-        mb_init(su32(&ms.q_full), 1);
-        mb_init(su32(&ms.q_free), 6);  // both issuers, and group 0's warps, which join over Q's memory
+        mb_init(su32(&ms.q_full[0]), 1);
+        mb_init(su32(&ms.q_full[1]), 1);
+        mb_init(su32(&ms.stagger), 4);
+        mb_init(su32(&ms.q_free), 10);  // both issuers, and the groups' warps, which join over Q's memory
         ms.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -134,19 +141,25 @@ __global__ void __launch_bounds__(XT, 1)
 
     if (warp == 0) {
         // ---- copies
-        uint32_t pos = 0, units = 0;
+        uint32_t pos = 0, units = 0, freed = 0;
+        int n_before = 0;
         bool ok = true;
         while (ok && share.next(p, sg)) {
             const int n = sg.t1 - sg.t0;
-            // Q: the rows of tile_nodes nodes, node by node, are one box; nodes past the last are zeros
-            if (units && !(ok = wait_all(ms.q_free, (units - 1) & 1))) break;
+            // Q: the rows of tile_nodes nodes, node by node, are one box; nodes past the last are zeros. Units
+            // of one tile row take the two places in turn, ahead of time after a unit of a single key tile
+            // (which needs no join over Q's memory).
+            const uint32_t before = units == 0 ? 0 : !two && n_before == 1 ? units - 1 : units;
+            for (; ok && freed < before; ++freed) ok = wait_all(ms.q_free, freed & 1);
+            if (!ok) break;
+            n_before = n;
             if (lane == 0) {
-                const uint32_t bar = su32(&ms.q_full);
+                const uint32_t bar = su32(&ms.q_full[units & 1]);
                 mb_expect(bar, (two ? 2 : 1) * (HD / 64) * 128 * tile_rows);
                 for (int w = 0; w < (two ? 2 : 1); ++w)
 #pragma unroll
                     for (int a = 0; a < HD / 64; ++a)
-                        tma_load_4d(s_q + w * TILE + a * ATOM, &tmq, 64 * a, sg.head * p.group,
+                        tma_load_4d(s_q + (two ? w : units & 1) * TILE + a * ATOM, &tmq, 64 * a, sg.head * p.group,
                                     row0 / p.group + w * p.tile_nodes, sg.seq, bar);
             }
             __syncwarp();
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(XT, 1)
             }
         }
         if (!ok && lane == 0) {  // leave no copy in flight
-            if (units) mb_wait(su32(&ms.q_full), (units - 1) & 1);
+            for (uint32_t u = units > 2 ? units - 2 : 0; u < units; ++u) mb_wait(su32(&ms.q_full[u & 1]), (u >> 1) & 1);
             for (uint32_t s = 0; s < ST && s < pos; ++s) mb_wait(su32(&ms.full[s]), ((pos - 1 - s) / ST) & 1);
         }
     } else if (warp == 1 || warp == 3) {
@@ -176,7 +189,7 @@ __global__ void __launch_bounds__(XT, 1)
         const int w = warp == 3, step = two ? 1 : 2;
         const bool leader = elect_one();
         const uint32_t t_s = tmem + 128 * w, t_o = tmem + 256 + 128 * w;
-        const uint64_t dq = umma_desc(s_q + (two ? w : 0) * TILE);
+        uint64_t dq = 0;
         uint32_t base = 0, done = 0, units = 0, ord = 0, landed = 0;
         bool ok = true;
         auto full = [&](uint32_t pos) {  // the tiles up to ring position pos
@@ -196,9 +209,14 @@ __global__ void __launch_bounds__(XT, 1)
         while (ok && share.next(p, sg)) {
             const int n = sg.t1 - sg.t0, first_tail = max(0, sg.past / KV_TILE - sg.t0);
             int i = two ? 0 : w;
-            if (!(ok = wait_all(ms.q_full, units & 1))) break;
+            if (!(ok = wait_all(ms.q_full[units & 1], (units >> 1) & 1))) break;
+            dq = umma_desc(s_q + (two ? w : units & 1) * TILE);
             if (i < n) {
                 const uint32_t k = base + pos_k(i);
+                // The groups of two row tiles share their key tiles and so would run in step, both reading
+                // scores and then both waiting for the special function unit: the second starts when the
+                // first has its first scores.
+                if (two && w == 1 && units == 0 && !(ok = wait_all(ms.stagger, 0))) break;
                 if (!(ok = full(k))) break;
                 tc_after_sync();
                 if (leader) {
@@ -277,22 +295,29 @@ __global__ void __launch_bounds__(XT, 1)
                 const int lo = max(0, sg.past - key0), hi = min(KV_TILE, n_keys - key0);  // the tree's rows here
                 uint4* v = reinterpret_cast<uint4*>(sm + SM::OFF_KV + (pos % ST) * TILE);
                 for (int a = 0; a < HD / 64; ++a, v += ATOM / 16) {
-                    for (int x = 8 * hi + lane; x < 8 * KV_TILE; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 8
-                    for (int x = 8 * lo + lane; x < 8 * hi; x += 32) {
-                        uint4 y = v[x];
+                    for (int x = 8 * hi + lane; x < 8 * KV_TILE; x += 32) v[x] = make_uint4(0u, 0u, 0u, 0u);
+                    for (int x0 = 8 * lo + lane; x0 < 8 * hi; x0 += 256) {
+                        uint4 y[8];
+                        uint32_t any = 0;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u) y[u] = x0 + 32 * u < 8 * hi ? v[x0 + 32 * u] : make_uint4(0u, 0u, 0u, 0u);
                         // an exponent of all ones carries into bit 15 of its half
-                        constexpr uint32_t ONE = BF ? 0x00800080u : 0x04000400u;
-                        if ((((y.x & 0x7FFF7FFFu) + ONE) | ((y.y & 0x7FFF7FFFu) + ONE) | ((y.z & 0x7FFF7FFFu) + ONE) |
-                             ((y.w & 0x7FFF7FFFu) + ONE)) & 0x80008000u) {
-                            uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+                        constexpr uint32_t ONE = BF ? 0x00800080u : 0x04000400u, ABS = 0x7FFF7FFFu;
+#pragma unroll
+                        for (int u = 0; u < 8; ++u)
+                            any |= ((y[u].x & ABS) + ONE) | ((y[u].y & ABS) + ONE) | ((y[u].z & ABS) + ONE) | ((y[u].w & ABS) + ONE);
+                        if (!(any & 0x80008000u)) continue;
+                        for (int x = x0; x < 8 * hi; x += 32) {  // to the end: what is clean stays as it is
+                            uint32_t* z = reinterpret_cast<uint32_t*>(v + x);
                             for (int e = 0; e < 4; ++e) {
-                                if (nonfinite2<BF>(w[e] & 0xFFFFu)) w[e] &= 0xFFFF0000u;
-                                if (nonfinite2<BF>(w[e] & 0xFFFF0000u)) w[e] &= 0xFFFFu;
+                                const uint32_t w = z[e];
+                                if (!nonfinite2<BF>(w)) continue;
+                                z[e] = (nonfinite2<BF>(w & 0xFFFFu) ? 0u : w & 0xFFFFu) | (nonfinite2<BF>(w & 0xFFFF0000u) ? 0u : w & 0xFFFF0000u);
+                                atomicOr(&bad[x >> 8], 1u << ((x >> 3) & 31));
                             }
-                            v[x] = y;
-                            atomicOr(&bad[x >> 8], 1u << ((x >> 3) & 31));
                         }
+                        break;
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -332,6 +357,7 @@ __global__ void __launch_bounds__(XT, 1)
                 for (int h = 0; h < 2; ++h) {
                     if (!(ok = wait_all(ms.s_full[w][h], done & 1))) break;
                     tc_after_sync();
+                    if (two && w == 0 && done == 0 && h == 0) arrive_warp(ms.stagger);
                     if (warp_on) {
                         uint32_t v[2][32];
 #pragma unroll
@@ -444,41 +470,44 @@ __global__ void __launch_bounds__(XT, 1)
             const bool whole = sg.t0 == 0 && sg.t1 == sg.tiles;
             const size_t orow = ((size_t)sg.seq * p.n_nodes + node) * p.n_heads + sg.head * p.group + head_in;
             float* part = ws.parts + ((size_t)blockIdx.x * 2 + (sg.t0 == 0 ? 1 : 0)) * part_floats(p.block_rows, HD);
+            // Alternate tiles: the groups hold two parts of the same rows. Each finishes one half of the columns,
+            // with the other group's values of that half passed through shared memory over Q: region w,
+            // [128][HD / 2], 16-byte chunk c of row r at c ^ (r & 7).
             const bool join = !two && n > 1;
-            float* js = reinterpret_cast<float*>(sm);  // [128][HD], 16-byte chunk c of row r at c ^ (r & 7), over Q
-            float f0 = 1.f, f1 = 0.f;
+            constexpr int HC = HD / 64;  // 32-column blocks of a half
+            float f0 = 1.f, f1 = 0.f;    // of this group's part and of the other's
             if (join) {
                 if (!(ok = meet())) break;  // both groups' MMAs over Q are done
-                if (w == 1) {
-                    if (warp_on) {
+                float* js = reinterpret_cast<float*>(sm) + w * 128 * (HD / 2) + r * (HD / 2);
+                if (warp_on) {
 #pragma unroll 1
-                        for (int c = 0; c < HD / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld32(t_o + 32 * c, o);
-                            tmem_wait_ld();
-                            tmem_pin32(o);
+                    for (int c = 0; c < HC; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + 32 * (c + (w ? 0 : HC)), o);
+                        tmem_wait_ld();
+                        tmem_pin32(o);
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                *reinterpret_cast<uint4*>(js + r * HD + (((8 * c + j) ^ (r & 7)) << 2)) =
-                                    make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                        }
-                        ms.jm[r] = m;
-                        ms.jl[r] = l;
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<uint4*>(js + (((8 * c + j) ^ (r & 7)) << 2)) =
+                                make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                     }
+                    ms.jm[w][r] = m;
+                    ms.jl[w][r] = l;
                 }
                 if (!(ok = meet())) break;
-                if (w == 0 && warp_on) {
-                    const float m1 = ms.jm[r], mj = fmaxf(m, m1), bj = mj == -INFINITY ? 0.f : mj;
+                if (warp_on) {
+                    const float m1 = ms.jm[w ^ 1][r], mj = fmaxf(m, m1), bj = mj == -INFINITY ? 0.f : mj;
                     f0 = ex2((m - bj) * c2);
                     f1 = ex2((m1 - bj) * c2);
-                    l = l * f0 + ms.jl[r] * f1;
+                    l = l * f0 + ms.jl[w ^ 1][r] * f1;
                     m = mj;
                 }
             }
-            if (warp_on && (two || w == 0)) {
+            if (warp_on && mine) {
                 const float inv = whole ? row_inv(l) : 1.f;
+                const float* js = reinterpret_cast<const float*>(sm) + (w ^ 1) * 128 * (HD / 2) + r * (HD / 2);
 #pragma unroll 1
-                for (int c = 0; c < HD / 32; ++c) {
+                for (int c = join && w ? HC : 0; c < (join && !w ? HC : 2 * HC); ++c) {
                     uint32_t o[32];
                     tmem_ld32(t_o + 32 * c, o);
                     tmem_wait_ld();
@@ -487,9 +516,10 @@ __global__ void __launch_bounds__(XT, 1)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(o[j]);
                     if (join) {
+                        const int cj = 8 * (c - (w ? HC : 0));
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const float4 y = *reinterpret_cast<const float4*>(js + r * HD + (((8 * c + j) ^ (r & 7)) << 2));
+                            const float4 y = *reinterpret_cast<const float4*>(js + (((cj + j) ^ (r & 7)) << 2));
                             x[4 * j] = x[4 * j] * f0 + y.x * f1;
                             x[4 * j + 1] = x[4 * j + 1] * f0 + y.y * f1;
                             x[4 * j + 2] = x[4 * j + 2] * f0 + y.z * f1;
@@ -512,7 +542,7 @@ __global__ void __launch_bounds__(XT, 1)
                                 make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
                     }
                 }
-                if (valid) {
+                if (valid && (two || w == 0)) {
                     if (whole) {
                         if (lse) lse[orow] = l == 0.f ? -INFINITY : m * p.scale + logf(l);
                     } else {
@@ -522,10 +552,8 @@ __global__ void __launch_bounds__(XT, 1)
                 }
             }
             tc_before_sync();
-            if (w == 0) {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                arrive_warp(ms.q_free);
-            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive_warp(ms.q_free);
         }
     }
     tc_before_sync();
