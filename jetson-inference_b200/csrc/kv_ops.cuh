@@ -123,15 +123,35 @@ constexpr int KV_TILE = 128;
 __device__ __forceinline__ int seq_tiles(const TreeParams& p, int past) {
     return (past + p.n_nodes + KV_TILE - 1) / KV_TILE;
 }
-// Shares of n groups (at most as many as tiles, so that none is empty and the parts of a unit are
-// those of consecutive groups): the first `more` take each + 1 tiles, the others `each`. The host
-// refuses shapes of 2^31 tiles and more.
+// Shares of n groups, none of them empty, so that the parts of a unit are those of consecutive groups.
+// In general the first `more` groups take each + 1 tiles, the others `each`. Short shares of units
+// that are all alike (one sequence) do not cross from one unit to the next: a group that finishes one
+// unit and begins another pays a whole unit's latency twice, 2 us, which a tile less per group does
+// not win back below about 16 tiles a group. Then a unit has `per` groups, part x of it tiles
+// unit_tiles x / per and on. The host refuses shapes of 2^31 tiles and more.
 struct Shares {
-    int n, each, more;
+    int n, each, more, per, unit_tiles;
     Shares() = default;
-    __device__ __forceinline__ Shares(int total, int groups) : n(min(groups, total)), each(total / n), more(total - each * n) {}
-    __device__ __forceinline__ int start(int g) const { return g * each + min(g, more); }
+    __device__ __forceinline__ Shares(int total, int groups, int tiles) {
+        n = min(groups, total);
+        each = total / n;
+        more = total - each * n;
+        unit_tiles = tiles;
+        const int units = tiles ? total / tiles : 0;
+        per = tiles && groups >= units && each < 16 ? min(groups / units, tiles) : 0;
+        if (per) n = per * units;
+    }
+    __device__ __forceinline__ int start(int g) const {
+        if (per) return g / per * unit_tiles + (int)((int64_t)unit_tiles * (g % per) / per);
+        return g * each + min(g, more);
+    }
     __device__ __forceinline__ int owner(int t) const {  // of tile t
+        if (per) {
+            const int u = t / unit_tiles, x = t - u * unit_tiles;
+            int g = (int)((int64_t)x * per / unit_tiles);
+            while (g + 1 < per && (int)((int64_t)unit_tiles * (g + 1) / per) <= x) ++g;
+            return u * per + g;
+        }
         return t < more * (each + 1) ? t / (each + 1) : more + (t - more * (each + 1)) / each;
     }
 };
@@ -202,7 +222,7 @@ __device__ __forceinline__ Share share_begin(const TreeParams& p, int g, int gro
     int sum = 0;
     for (int s = threadIdx.x & 31; s < p.n_seqs; s += 32) sum += seq_tiles(p, clamped_past(p, s));
     sum = (int)__reduce_add_sync(JINF_FULL_MASK, (unsigned)sum);
-    all = Shares(sum * p.n_kv_heads, groups);
+    all = Shares(sum * p.n_kv_heads, groups, p.n_seqs == 1 ? sum : 0);
     Share sh{0, 0, 0, 0};
     if (g >= all.n) return sh;
     const int begin = all.start(g);

@@ -352,7 +352,12 @@ __global__ void __launch_bounds__(XT, 1)
             float m = -INFINITY, l = 0.f;
             for (int i = two ? 0 : w; i < n; i += step) {
                 const bool tail = i >= first_tail;
-                const int u0 = (sg.t0 + i) * KV_TILE - sg.past;
+                uint32_t see[4];  // the tile's keys that the row sees, loaded before its scores are waited for
+                if (tail && warp_on) {
+                    const int u0 = (sg.t0 + i) * KV_TILE - sg.past;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) see[c] = seen_keys(p, mask, node, u0 + 32 * c);
+                }
 #pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
                     if (!(ok = wait_all(ms.s_full[w][h], done & 1))) break;
@@ -368,10 +373,10 @@ __global__ void __launch_bounds__(XT, 1)
                         if (tail) {
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                const uint32_t see = seen_keys(p, mask, node, u0 + 64 * h + 32 * c);
+                                const uint32_t w32 = h ? see[2 + c] : see[c];
 #pragma unroll
                                 for (int j = 0; j < 32; ++j)
-                                    if (!((see >> j) & 1u)) v[c][j] = 0xFF800000u;
+                                    if (!((w32 >> j) & 1u)) v[c][j] = 0xFF800000u;
                             }
                         }
                         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
