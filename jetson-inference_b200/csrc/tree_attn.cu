@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(TW * 32, 1)
     }
     __syncthreads();
     Share share = s_share;
-    const TreeWs ws = tree_ws(workspace, gridDim.x);
+    const TreeWs ws = tree_ws(workspace);
     const float c2 = p.scale * LOG2E;
 
     for (Segment u; share.next(p, u);) {
@@ -334,7 +334,7 @@ cudaError_t launch_rows(const TreeParams& p, const TreePlan& plan, uint16_t* out
 
 size_t tree_workspace_bytes(const TreePlan& plan, int head_dim) {
     const int ctas = plan.n_groups * plan.row_blocks;
-    return tree_ws_head(ctas) + sizeof(float) * (size_t)ctas * 2 * part_floats(plan.block_rows, head_dim);
+    return TREE_WS_HEAD + sizeof(float) * (size_t)ctas * 2 * part_floats(plan.block_rows, head_dim);
 }
 
 TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_past, int sms, bool mma_fits) {
@@ -359,7 +359,8 @@ TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_p
 cudaError_t tree_attn_launch(const TreeParams& p, const TreePlan& plan, bool bf, int head_dim, void* out, float* lse,
                              void* ws, cudaStream_t s) {
     uint16_t* o = (uint16_t*)out;
-    if (plan.n_groups < 1) return cudaErrorInvalidValue;  // fewer SMs than row blocks
+    if (plan.n_groups < 1 || plan.n_groups * plan.row_blocks > TREE_MAX_CTAS)
+        return cudaErrorInvalidValue;  // fewer SMs than row blocks, or more than there are counters
     if (plan.mma) return tree_mma_launch(p, plan, bf, head_dim, o, lse, ws, s);
     if (head_dim == 64) return bf ? launch_rows<true, 64>(p, plan, o, lse, ws, s) : launch_rows<false, 64>(p, plan, o, lse, ws, s);
     return bf ? launch_rows<true, 128>(p, plan, o, lse, ws, s) : launch_rows<false, 128>(p, plan, o, lse, ws, s);

@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(XT, 1)
     const int row0 = block * p.block_rows, rows = min(p.block_rows, p.n_rows - row0);
     const int tile_rows = p.tile_nodes * p.group;
     const bool two = rows > tile_rows;  // two row tiles, one per softmax group; else alternate key tiles
-    const TreeWs ws = tree_ws(workspace, gridDim.x);
+    const TreeWs ws = tree_ws(workspace);
 
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {

@@ -27,13 +27,14 @@ struct TreeWs {
     unsigned* count;  // [CTAs] of the unit that CTA c begins: n parts announced, then n times seen, then 0 again
     float* parts;
 };
-__host__ __device__ __forceinline__ size_t tree_ws_head(int n_ctas) {  // bytes before the slots
-    return ((size_t)n_ctas * 4 + 255) & ~(size_t)255;
-}
-__host__ __device__ __forceinline__ TreeWs tree_ws(void* ws, int n_ctas) {
+// Counters come first and take the same room whatever the launch, so that calls of other shapes may
+// share a workspace: what one leaves in its slots never lies where another counts.
+constexpr int TREE_MAX_CTAS = 1024;
+constexpr size_t TREE_WS_HEAD = TREE_MAX_CTAS * sizeof(unsigned);
+__host__ __device__ __forceinline__ TreeWs tree_ws(void* ws) {
     TreeWs w;
     w.count = (unsigned*)ws;
-    w.parts = (float*)((uint8_t*)ws + tree_ws_head(n_ctas));
+    w.parts = (float*)((uint8_t*)ws + TREE_WS_HEAD);
     return w;
 }
 

@@ -1,0 +1,220 @@
+"""Speculative decoding with a draft tree over a bounded cache, with the operators of
+include/jinf/kv_ops.h: one step verifies a whole tree of drafted tokens, keeps the accepted path, credits
+the cached rows with the attention it paid them, and cuts the cache back when it is full.
+
+    python -m jinf.tree_decode [--tokens N] [--nodes T] [--right P] [--keep R] [--limit R] [--model 8b|tiny]
+
+The model is a small stand-in (random attention layers with the head layout of the named shape, and an
+embedding that is also the output head); its drafts are its own greedy continuations, each right
+with probability P, as a draft model's would be. `TreeCache` is the part that a caller with a model of
+its own would take over.
+"""
+from __future__ import annotations
+
+import argparse
+import time
+
+import torch
+
+from . import kernels as K
+from .model import LLAMA3_8B, TINY
+
+
+class TreeCache:
+    """The K/V caches of all layers of one sequence (layers are the views' first axis), their rows'
+    attention weight, and the step that a verified draft tree takes through them."""
+
+    def __init__(self, n_layers, n_heads, n_kv_heads, head_dim, max_ctx, max_nodes, dtype=torch.float16, device="cuda"):
+        self.n_heads, self.max_ctx, self.max_nodes = n_heads, max_ctx, max_nodes
+        self.k = torch.zeros(n_layers, n_kv_heads, max_ctx, head_dim, dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.mass = torch.zeros(n_layers, n_kv_heads, max_ctx, device=device)
+        self.all = K.KvView(self.k, self.v)                                         # for commit and eviction
+        self.layer = [K.KvView(self.k[i], self.v[i]) for i in range(n_layers)]      # for attention
+        self.n = 0                                                                  # cached rows (host)
+        self.n_rows = torch.zeros(n_layers, dtype=torch.int32, device=device)       # the same on the device
+        self.max_past = max_ctx - max_nodes
+        ws = max(K.tree_attention_workspace_bytes(self.layer[0], n_heads, t, self.max_past) for t in (1, max_nodes))
+        self.workspace = torch.zeros(ws, dtype=torch.uint8, device=device)
+        self.queries = []                                                           # of the step, per layer
+
+    def attend(self, i, q, k, v, mask):
+        """Layer i's attention of the step's nodes (q [T, H, hd], k and v [T, Hkv, hd]); mask: K.tree_mask's."""
+        t = q.shape[0]
+        self.k[i, :, self.n:self.n + t] = k.transpose(0, 1)
+        self.v[i, :, self.n:self.n + t] = v.transpose(0, 1)
+        out, lse = torch.empty_like(q), torch.empty(t, self.n_heads, device=q.device)
+        K.tree_attention(out, q, self.layer[i], self.n_rows[:1], self.max_past, self.workspace, mask=mask, lse=lse)
+        self.queries.append((q, lse))
+        return out
+
+    def accept(self, path, mask):
+        """Ends the step with the accepted nodes (ascending): their attention weight is credited, their rows
+        are kept, the other nodes' rows are dropped."""
+        t = self.queries[0][0].shape[0]
+        weight = torch.zeros(1, t)
+        weight[0, path] = 1.0
+        weight = weight.to(self.k.device)
+        for i, (q, lse) in enumerate(self.queries):
+            K.attention_mass(self.mass[i:i + 1], q, self.layer[i], self.n_rows[:1], self.max_past, lse, mask=mask,
+                             node_weight=weight)
+        self.queries.clear()
+        layers = self.k.shape[0]
+        nodes = torch.tensor([path], dtype=torch.int32).repeat(layers, 1).to(self.k.device)
+        count = torch.full((layers,), len(path), dtype=torch.int32, device=self.k.device)
+        after = torch.empty_like(self.n_rows)
+        K.tree_commit(self.all, self.mass, self.n_rows, self.max_past, nodes, count, t, after)
+        self.n_rows, self.n = after, self.n + len(path)
+
+    def evict(self, keep, sink, recent):
+        """Cuts every layer and head back to `keep` rows, in place."""
+        ids = torch.empty(*self.mass.shape[:2], keep, dtype=torch.int32, device=self.k.device)
+        after = torch.empty_like(self.n_rows)
+        K.kv_evict(self.all, None, self.mass, self.mass, self.n_rows, ids, after, keep, sink, recent)
+        self.n_rows, self.n = after, min(self.n, keep)
+        return ids
+
+
+def rotate(x, pos, base):
+    """Rotary positions, adjacent pairs: x [T, H, hd], pos [T]."""
+    half = x.shape[-1] // 2
+    f = base ** (-torch.arange(half, device=x.device, dtype=torch.float32) / half)
+    a = pos.float()[:, None, None] * f
+    x = x.float().unflatten(-1, (half, 2))
+    y = torch.stack((x[..., 0] * a.cos() - x[..., 1] * a.sin(), x[..., 0] * a.sin() + x[..., 1] * a.cos()), -1)
+    return y.flatten(-2)
+
+
+class StandIn:
+    """Attention layers of random weights with a residual, an embedding tied to the output head."""
+
+    def __init__(self, shape, n_layers=2, n_vocab=512, dtype=torch.float16, seed=0):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        self.shape, self.dtype, self.n_layers = shape, dtype, n_layers
+        d, hd = shape.n_embd, shape.head_dim
+        rnd = lambda *s: (torch.randn(*s, generator=g, device="cuda") * s[-1] ** -0.5).to(dtype)  # noqa: E731
+        self.embed = torch.nn.functional.normalize(rnd(n_vocab, d).float(), dim=1).mul(d ** 0.5).to(dtype)
+        self.wq = [rnd(shape.n_heads * hd, d) for _ in range(n_layers)]
+        self.wk = [rnd(shape.n_heads_kv * hd, d) for _ in range(n_layers)]
+        self.wv = [rnd(shape.n_heads_kv * hd, d) for _ in range(n_layers)]
+        self.wo = [rnd(d, shape.n_heads * hd) * 4 for _ in range(n_layers)]
+
+    def step(self, tokens, positions, attend):
+        """Logits [T, vocab] of T tokens; attend(i, q, k, v) is the attention."""
+        s, t = self.shape, len(tokens)
+        dev = self.embed.device
+        h = self.embed[torch.tensor(tokens, device=dev)].float()
+        pos = torch.tensor(positions, device=dev)
+        for i in range(self.n_layers):
+            x = torch.nn.functional.rms_norm(h, h.shape[-1:]).to(self.dtype)
+            q = rotate((x @ self.wq[i].T).view(t, s.n_heads, -1), pos, s.rope_freq_base).to(self.dtype)
+            k = rotate((x @ self.wk[i].T).view(t, s.n_heads_kv, -1), pos, s.rope_freq_base).to(self.dtype)
+            v = (x @ self.wv[i].T).view(t, s.n_heads_kv, -1)
+            h = h + (attend(i, q, k, v).reshape(t, -1) @ self.wo[i].T).float()
+        # a token's own embedding is left out of its successor's score, or it would always repeat itself
+        h = torch.nn.functional.rms_norm(h, h.shape[-1:])
+        e = self.embed.float()
+        logits = h @ e.T
+        own = torch.tensor(tokens, device=dev)
+        return logits.scatter_(1, own[:, None], -1e30)
+
+
+def draft_tree(rng, root, guess, nodes, right, n_vocab):
+    """A tree whose node 0 is the last accepted token: a chain of guesses and wrong siblings beside it.
+    Returns tokens, parents, depths. guess: the tokens a good draft model would propose, in order."""
+    tokens, parents, depth = [root], [-1], [0]
+    tip = 0
+    for good in guess:
+        if len(tokens) >= nodes:
+            break
+        kids = [int(rng.integers(n_vocab)) for _ in range(2)]
+        if rng.random() < right:
+            kids[int(rng.integers(2))] = good
+        first = len(tokens)
+        for x in kids[:nodes - first]:
+            tokens.append(x)
+            parents.append(tip)
+            depth.append(depth[tip] + 1)
+        here = [first + j for j, x in enumerate(kids) if first + j < nodes and x == good]
+        if not here:
+            break
+        tip = here[0]
+    return tokens, parents, depth
+
+
+def decode(model, prompt, n_tokens, nodes=16, right=0.7, limit=384, keep=256, sink=4, recent=64, seed=0, check=None):
+    """Greedy decoding of n_tokens after `prompt` with draft trees. Returns the tokens and the steps taken.
+    check(accepted tokens, logits): called per step."""
+    import numpy as np
+    rng = np.random.default_rng(seed)
+    s = model.shape
+    cache = TreeCache(model.n_layers, s.n_heads, s.n_heads_kv, s.head_dim, limit + nodes, max(nodes, len(prompt)))
+    # the prompt but its last token: a chain of nodes, all accepted
+    body = prompt[:-1]
+    if body:
+        model.step(body, range(len(body)), lambda i, q, k, v: cache.attend(i, q, k, v, None))
+        cache.accept(list(range(len(body))), None)
+    out, position, last, steps = [], len(body), prompt[-1], 0
+    while len(out) < n_tokens:
+        # the stand-in's draft model: the greedy continuation itself, seen through a copy of the cache
+        guess = greedy(model, cache, last, position, 6)
+        tokens, parents, depth = draft_tree(rng, last, guess, nodes, right, model.embed.shape[0])
+        mask = K.tree_mask(parents).to(model.embed.device)
+        logits = model.step(tokens, [position + d for d in depth], lambda i, q, k, v: cache.attend(i, q, k, v, mask))
+        best = logits.argmax(1).tolist()
+        path = [0]  # node 0, the token already chosen; then every drafted child that the model chose too
+        while True:
+            kids = [t for t in range(len(tokens)) if parents[t] == path[-1] and tokens[t] == best[path[-1]]]
+            if not kids:
+                break
+            path.append(kids[0])
+        got = [tokens[t] for t in path[1:]] + [best[path[-1]]]
+        if check:
+            check(cache, tokens, parents, path, logits)
+        cache.accept(path, mask)
+        out += got
+        position += len(path)
+        last, steps = got[-1], steps + 1
+        if cache.n + nodes > limit:
+            cache.evict(keep, sink, recent)
+    return out[:n_tokens], steps
+
+
+def greedy(model, cache, token, position, n):
+    """n greedy tokens one at a time, over scratch rows behind the cached ones (nothing is kept)."""
+    out, at = [], cache.n
+    for j in range(n):
+        if cache.n + 1 > cache.max_past:
+            break
+        logits = model.step([token], [position + j], lambda i, q, k, v: cache.attend(i, q, k, v, None))
+        cache.queries.clear()
+        cache.n += 1
+        cache.n_rows = cache.n_rows + 1
+        token = int(logits.argmax())
+        out.append(token)
+    cache.n_rows = cache.n_rows - (cache.n - at)
+    cache.n = at
+    return out
+
+
+def main() -> None:
+    ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
+    ap.add_argument("--tokens", type=int, default=300)
+    ap.add_argument("--nodes", type=int, default=16)
+    ap.add_argument("--right", type=float, default=0.8)
+    ap.add_argument("--limit", type=int, default=384)
+    ap.add_argument("--keep", type=int, default=256)
+    ap.add_argument("--model", choices=("8b", "tiny"), default="tiny")
+    a = ap.parse_args()
+    model = StandIn(TINY if a.model == "tiny" else LLAMA3_8B)
+    t = time.perf_counter()
+    out, steps = decode(model, [1, 2, 3, 4, 5, 6, 7, 8], a.tokens, a.nodes, a.right, a.limit, a.keep)
+    torch.cuda.synchronize()
+    K.kv_ops_status()
+    print(f"{len(out)} tokens in {steps} verified trees ({len(out) / steps:.2f} a tree), cache of {a.keep} to {a.limit} rows, "
+          f"{time.perf_counter() - t:.2f} s with the stand-in's drafts; first tokens {out[:8]}")
+
+
+if __name__ == "__main__":
+    main()

@@ -481,3 +481,49 @@ def test_long_caches_many_tiles_per_cta(cuda, dtype, hd, nh, nkv, nodes, lengths
             assert bool(((m.double() - want).abs() <= 1e-4 * add + 2.0 ** -22 * want.abs()).all())
         assert torch.equal(o, out) and torch.equal(e, lse) and torch.equal(m, first)
     K.kv_ops_status()
+
+
+def test_tree_decode_example(cuda):
+    """The example's steps against the same model in 32 bits with its attention written out: the logits of the
+    accepted nodes over the rows that the cache kept, and as many accepted tokens as a good draft brings."""
+    from jinf import tree_decode as E
+    from jinf.model import TINY
+    model = E.StandIn(TINY, seed=3)
+    seen = []
+
+    def check(cache, tokens, parents, path, logits):
+        # the last accepted node again, in plain torch: cached rows, then the path's own rows
+        n, group = cache.n, TINY.n_heads // TINY.n_heads_kv
+        rows = list(range(n)) + [n + t for t in path]
+        for i, (q, lse) in enumerate(cache.queries):
+            k, v = cache.k[i][:, rows].float(), cache.v[i][:, rows].float()
+            qq = q[path[-1]].float().view(TINY.n_heads_kv, group, -1)
+            s = torch.einsum("hgd,hrd->hgr", qq, k) * TINY.head_dim ** -0.5
+            want = torch.logsumexp(s, -1).flatten()
+            assert torch.allclose(lse[path[-1]], want, atol=1e-3)
+        seen.append((n, len(path)))
+
+    out, steps = E.decode(model, list(range(1, 9)), 250, nodes=12, right=0.9, limit=160, keep=96, recent=32, check=check)
+    assert len(out) == 250 and steps < 200
+    assert max(n for n, _ in seen) <= 160 and min(n for n, _ in seen[20:]) >= 96
+
+
+def test_one_workspace_for_calls_of_several_shapes(cuda):
+    """Calls of other node counts, and of both kernels, in turn over one workspace of the largest's size."""
+    from jinf import kernels as K
+    g = gen(55)
+    k, v = make_cache(g, 1, 4, 3000, 128, F16)
+    kv = K.KvView(k, v)
+    n_past = torch.tensor([2500], dtype=torch.int32, device="cuda")
+    ws = torch.zeros(max(K.tree_attention_workspace_bytes(kv, 16, t, 2600) for t in (1, 3, 40, 70)), dtype=torch.uint8,
+                     device="cuda")
+    want = {}
+    for t in (40, 1, 70, 3, 1, 40, 3, 70):
+        q = torch.randn(1, t, 16, 128, generator=gen(t), device="cuda", dtype=F16)
+        out, lse = torch.empty_like(q), torch.empty(1, t, 16, device="cuda")
+        K.tree_attention(out, q, kv, n_past, 2600, ws, lse=lse)
+        if t in want:
+            assert torch.equal(out, want[t])
+        else:
+            check_attention(q, k, v, n_past, out, lse, [None], 128 ** -0.5)
+        want[t] = out
