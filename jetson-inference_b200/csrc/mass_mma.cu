@@ -4,18 +4,19 @@
 // S^T = K Q^T with keys as the MMA's 128 rows and up to 128 query rows as its columns: in tensor
 // memory a lane is a key, so its sum over the query rows needs no exchange between threads. What
 // bounds it: K from HBM while the query rows are few; the exponentials (16 a cycle and SM) when
-// there are hundreds. A CTA takes a share of the key tiles (kv_ops.cuh); per up to 4 tiles of
-// a kv head, kept in shared memory, it runs over the query rows 128 at a time:
-//   warp 0      copies K tiles (TMA);
-//   warps 1, 2  issue the MMAs into four score buffers of 128 columns, in turn: one issuer's turn (waits
-//               and eight MMAs, 1200 cycles) is longer than the exponentials of a buffer (1024);
-//   warp 3      brings 128 query rows into one of two stages, with the exponent's constant of each
+// there are hundreds. A CTA takes a share of the key tiles (kv_ops.cuh) with three independent
+// lanes, each a key tile in shared memory, a score buffer in tensor memory, an issuing warp and four
+// summing warps; query rows pass all lanes 128 at a time through a ring of three stages:
+//   warp 0      brings query rows into the ring, with the exponent's constant of each
 //               (w e^(s - lse) = 2^(s log2 e + log2 w - lse log2 e)):
 //               boxes of whole nodes by TMA when every node counts and nodes fill a stage evenly, else
 //               the rows of weight > 0 one by one (16-byte asynchronous copies into the 128B-swizzled
 //               layout; about 4000 cycles a stage where the boxes take 1500);
-//   warps 4-11  two groups, one thread per key, one group per tile parity: 64 columns of two tiles into
-//               registers, then w e^(s - lse) added up. A key's sum has one owner and one order.
+//   warps 1-3   one a lane: copies the lane's key tiles (TMA) and issues its MMAs;
+//   warps 4-15  four a lane, one thread per key: 64 columns at a time into registers, then added up.
+// Three lanes out of step keep the special function unit busy through each other's waits and reads
+// (two groups in step left it idle half of the time); with the constants alone read from shared memory,
+// a broadcast word a score, that memory stays below it.
 // Every wait is bounded; one that runs out sets the error word and ends the CTA.
 #include "kv_ops.cuh"
 #include "umma.cuh"
@@ -25,33 +26,32 @@
 namespace jinf {
 namespace {
 
-constexpr int XT = 384;
+constexpr int XT = 512;
 constexpr int ATOM = 16384;  // 128 rows x 64 columns, 128B-swizzled
-constexpr int KT = 4;        // key tiles kept while the query rows pass; also the ring of K tiles
-constexpr int NB = 4;        // score buffers
-constexpr int NR = 4;        // stages whose row factors are kept: the MMAs run ahead of the sums
-constexpr int GROUPS = 2;
+constexpr int LANES = 3;
+constexpr int QS = 3;        // stages of query rows
+constexpr int NR = 4;        // stages whose row constants are kept: the MMAs run ahead of the sums
 constexpr int MASK_WORDS = JINF_TREE_MAX_NODES / 32, MASK_PITCH = MASK_WORDS + 1;  // odd: no bank conflicts down the rows
 
 template <int HD>
 struct MassMma {
     static constexpr int TILE = ATOM * (HD / 64);
-    static constexpr int OFF_Q = KT * TILE;
-    static constexpr int OFF_MISC = OFF_Q + 2 * TILE;
+    static constexpr int OFF_Q = LANES * TILE;
+    static constexpr int OFF_MISC = OFF_Q + QS * TILE;
     struct Misc {
-        uint64_t k_full[KT], k_free[KT], q_full[2], q_free[2], r_full[NR], r_free[NR], s_full[NB], s_free[NB], stagger, drain[2];
+        uint64_t k_full[LANES], k_free[LANES], q_full[QS], q_free[QS], r_full[NR], r_free[NR], s_full[LANES], s_free[LANES],
+            drain[LANES];
         Share share;
         uint32_t tmem;
         int abort;
         alignas(16) float bias[NR][128];    // of a stage's query rows: log2(weight) - lse log2 e
         uint32_t seen[NR][128][MASK_PITCH];  // where the stage meets tree rows: those that each row's node sees
-        uint8_t node[JINF_TREE_MAX_NODES];  // nodes of weight > 0, ascending (warp 3's)
+        uint8_t node[JINF_TREE_MAX_NODES];  // nodes of weight > 0, ascending (warp 0's)
     };
     static constexpr int TOTAL = OFF_MISC + (int)sizeof(Misc) + 1024;
 };
 static_assert(MassMma<128>::TOTAL + 64 <= 232448, "shared memory");
 static_assert(JINF_TREE_MAX_NODES <= 256, "node numbers are kept in bytes");
-static_assert(GROUPS == 2 && NB == 4 && KT == 4, "two buffers, an issuer and a group per tile parity");
 
 // Nodes of weight > 0, by a whole warp; their numbers, ascending, to `list` where it is not null.
 __device__ __forceinline__ int active_nodes(const TreeParams& p, const float* weight, int seq, uint8_t* list) {
@@ -106,24 +106,21 @@ __global__ void __launch_bounds__(XT, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < KT; ++i) {
+        for (int i = 0; i < LANES; ++i) {
             mb_init(su32(&ms.k_full[i]), 1);
-            mb_init(su32(&ms.k_free[i]), 2);
+            mb_init(su32(&ms.k_free[i]), 1);
+            mb_init(su32(&ms.s_full[i]), 1);
+            mb_init(su32(&ms.s_free[i]), 4);
+            mb_init(su32(&ms.drain[i]), 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < QS; ++i) {
             mb_init(su32(&ms.q_full[i]), 1);
-            mb_init(su32(&ms.q_free[i]), 2);
+            mb_init(su32(&ms.q_free[i]), LANES);
         }
         for (int i = 0; i < NR; ++i) {
             mb_init(su32(&ms.r_full[i]), 1);
-            mb_init(su32(&ms.r_free[i]), 4 * GROUPS);
+            mb_init(su32(&ms.r_free[i]), 4 * LANES);
         }
-        for (int i = 0; i < NB; ++i) {
-            mb_init(su32(&ms.s_full[i]), 1);
-            mb_init(su32(&ms.s_free[i]), 4);
-        }
-        mb_init(su32(&ms.stagger), 4);
-        for (int i = 0; i < 2; ++i) mb_init(su32(&ms.drain[i]), 1);
         ms.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -144,89 +141,18 @@ __global__ void __launch_bounds__(XT, 1)
     Segment sg;
 
     // A wait by parity tells phase x only from x - 1, so each role waits for every phase of a barrier
-    // in order (a score buffer belongs to the issuer and the group of its tile's parity).
+    // in order; a lane's barriers are its own.
     auto wait = [&](uint64_t& bar, uint32_t parity) { return mb_wait_warp(su32(&bar), parity, &ms.abort, p.err); };
     auto arrive_warp = [&](uint64_t& bar) {
         __syncwarp();
         if (lane == 0) mb_arrive(su32(&bar));
     };
-    // Every role walks the same loops: segments, then sets of key tiles, for each set stages of 128 query
-    // rows, for each stage the set's tiles, a score buffer per (stage, tile). With
-    // several stages a set is up to KT tiles, which stay while the rows pass; with one the rows stay.
-    auto set_of = [&](int stages) { return stages == 1 ? INT32_MAX : KT; };
+    // Every role walks the same loops: segments, then sets of key tiles, for each set the stages of 128
+    // query rows ("fills" of the ring). With several stages a set is one tile a lane, which stays while
+    // the rows pass; with one it is the whole segment, and the rows stay.
+    auto set_of = [&](int stages) { return stages == 1 ? INT32_MAX : LANES; };
 
     if (warp == 0) {
-        uint32_t pos = 0;
-        bool ok = true;
-        while (ok && share.next(p, sg)) {
-            if (active_nodes(p, weight, sg.seq, nullptr) == 0) continue;
-            for (int t = sg.t0; t < sg.t1; ++t, ++pos) {
-                const uint32_t slot = pos % KT;
-                if (pos >= KT && !(ok = wait(ms.k_free[slot], (pos / KT - 1) & 1))) break;
-                if (lane == 0) {
-                    const uint32_t bar = su32(&ms.k_full[slot]);
-                    mb_expect(bar, TILE);
-#pragma unroll
-                    for (int a = 0; a < HD / 64; ++a)
-                        tma_load_4d(s_k + slot * TILE + a * ATOM, &tmk, 64 * a, t * KV_TILE, sg.head, sg.seq, bar);
-                }
-                __syncwarp();
-            }
-        }
-        if (!ok && lane == 0)  // leave no copy in flight
-            for (uint32_t s = 0; s < KT && s < pos; ++s) mb_wait(su32(&ms.k_full[s]), ((pos - 1 - s) / KT) & 1);
-    } else if (warp < 3) {
-        const int turn = warp - 1;  // tiles of this parity
-        const bool leader = elect_one();
-        uint32_t pos = 0, fill = 0, mine = 0;
-        bool ok = true;
-        while (ok && share.next(p, sg)) {
-            const int rows = active_nodes(p, weight, sg.seq, nullptr) * p.group, stages = (rows + 127) / 128;
-            if (rows == 0) continue;
-            // With several stages the exponentials bind: the second group starts half a stage after the first,
-            // so that one's waits and reads fall into the other's sums instead of leaving both waiting.
-            if (turn && mine == 0 && stages > 1 && !(ok = wait(ms.stagger, 0))) break;
-            for (int t = sg.t0; ok && t < sg.t1;) {
-                const int n = min(set_of(stages), sg.t1 - t);
-                for (int st = 0; ok && st < stages; ++st, ++fill) {
-                    if (!(ok = wait(ms.q_full[fill & 1], (fill >> 1) & 1))) break;
-                    const int cols = min(128, (rows - 128 * st + 31) & ~31);
-                    const uint32_t idesc = umma_idesc(BF, 128, 0, false) | ((uint32_t)(cols >> 3) << 17);
-                    const uint64_t dq = umma_desc(s_q + (fill & 1) * TILE);
-                    for (int j = 0; ok && j < n; ++j) {
-                        const uint32_t slot = (pos + j) % KT;
-                        if (st == 0 && !(ok = wait(ms.k_full[slot], ((pos + j) / KT) & 1))) break;
-                        if ((j & 1) == turn) {
-                            const uint32_t b = turn + 2 * (mine & 1);
-                            if (mine >= 2 && !(ok = wait(ms.s_free[b], ((mine >> 1) - 1) & 1))) break;
-                            ++mine;
-                            tc_after_sync();
-                            if (leader) {
-                                const uint64_t dk = umma_desc(s_k + slot * TILE);
-#pragma unroll
-                                for (int kk = 0; kk < HD / 16; ++kk) {
-                                    const uint32_t off = ((kk >> 2) * ATOM + (kk & 3) * 32) >> 4;
-                                    umma_ss(tmem + 128 * b, dk + off, dq + off, idesc, kk > 0);
-                                }
-                                umma_commit(su32(&ms.s_full[b]));
-                            }
-                        }
-                        if (st == stages - 1 && leader) umma_commit(su32(&ms.k_free[slot]));
-                        __syncwarp();
-                    }
-                    if (!ok) break;
-                    if (leader) umma_commit(su32(&ms.q_free[fill & 1]));
-                    __syncwarp();
-                }
-                pos += n;
-                t += n;
-            }
-        }
-        if (!ok && leader) {  // the MMAs already issued finish before the memory goes
-            umma_commit(su32(&ms.drain[turn]));
-            mb_wait(su32(&ms.drain[turn]), 0);
-        }
-    } else if (warp == 3) {
         uint8_t* list = ms.node;
         uint32_t fill = 0, boxed = 0;
         bool ok = true;
@@ -236,7 +162,7 @@ __global__ void __launch_bounds__(XT, 1)
             if (rows == 0) continue;
             const uint32_t* mask = p.mask ? p.mask + sg.seq * p.mask_seq : nullptr;
             const bool boxes = rows == p.n_rows && 128 % p.group == 0;
-            const int fills = stages > 1 ? (sg.t1 - sg.t0 + KT - 1) / KT * stages : 1;
+            const int fills = stages > 1 ? (sg.t1 - sg.t0 + LANES - 1) / LANES * stages : 1;
             // lane l has rows l, l + 32, ..: where they are (-1: zeros), constant, node
             int64_t from[4];
             float bias[4];
@@ -267,10 +193,10 @@ __global__ void __launch_bounds__(XT, 1)
             };
             rows_of(0);
             for (int x = 0; x < fills; ++x) {
-                const uint32_t f = fill + x, s = f & 1;
-                const int cols = min(128, (rows - 128 * (x % stages) + 31) & ~31), rs = f % NR;
+                const uint32_t f = fill + x, s = f % QS;
+                const int cols = min(128, (rows - 128 * (x % stages) + 63) & ~63), rs = f % NR;
                 // the set's tiles, or with one stage all of the segment's, reach the tree's rows
-                const bool meets = (stages > 1 ? min(sg.t1, sg.t0 + (x / stages + 1) * KT) : sg.t1) * KV_TILE > sg.past;
+                const bool meets = (stages > 1 ? min(sg.t1, sg.t0 + (x / stages + 1) * LANES) : sg.t1) * KV_TILE > sg.past;
                 if (f >= NR && !(ok = wait(ms.r_free[rs], (f / NR - 1) & 1))) break;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -284,7 +210,7 @@ __global__ void __launch_bounds__(XT, 1)
                     }
                 }
                 arrive_warp(ms.r_full[rs]);
-                if (f >= 2 && !(ok = wait(ms.q_free[s], ((f >> 1) - 1) & 1))) break;
+                if (f >= QS && !(ok = wait(ms.q_free[s], (f / QS - 1) & 1))) break;
                 const uint32_t dst = s_q + s * TILE;
                 if (boxes) {
                     if (lane == 0) {
@@ -316,10 +242,70 @@ __global__ void __launch_bounds__(XT, 1)
             fill += fills;
         }
         if (!ok && lane == 0)  // leave no copy in flight
-            for (uint32_t f = boxed > 2 ? boxed - 2 : 0; f < boxed; ++f) mb_wait(su32(&ms.q_full[f & 1]), (f >> 1) & 1);
+            for (uint32_t f = boxed > QS ? boxed - QS : 0; f < boxed; ++f) mb_wait(su32(&ms.q_full[f % QS]), (f / QS) & 1);
+    } else if (warp <= LANES) {
+        const int g = warp - 1;
+        const bool leader = elect_one();
+        const uint32_t t_s = tmem + 128 * g;
+        const uint64_t dk = umma_desc(s_k + g * TILE);
+        uint32_t fill = 0, loads = 0, mine = 0;
+        bool ok = true;
+        while (ok && share.next(p, sg)) {
+            const int rows = active_nodes(p, weight, sg.seq, nullptr) * p.group, stages = (rows + 127) / 128;
+            if (rows == 0) continue;
+            auto load = [&](int t) {  // key tile t, once the lane's place is free
+                if (loads && !(ok = wait(ms.k_free[g], (loads - 1) & 1))) return;
+                ++loads;
+                if (leader) {
+                    const uint32_t bar = su32(&ms.k_full[g]);
+                    mb_expect(bar, TILE);
+#pragma unroll
+                    for (int a = 0; a < HD / 64; ++a)
+                        tma_load_4d(s_k + g * TILE + a * ATOM, &tmk, 64 * a, t * KV_TILE, sg.head, sg.seq, bar);
+                }
+                __syncwarp();
+            };
+            if (sg.t0 + g < sg.t1) load(sg.t0 + g);
+            for (int t = sg.t0; ok && t < sg.t1;) {
+                const int n = min(set_of(stages), sg.t1 - t);
+                for (int st = 0; ok && st < stages; ++st, ++fill) {
+                    const uint32_t s = fill % QS;
+                    if (!(ok = wait(ms.q_full[s], (fill / QS) & 1))) break;
+                    const int cols = min(128, (rows - 128 * st + 63) & ~63);
+                    const uint32_t idesc = umma_idesc(BF, 128, 0, false) | ((uint32_t)(cols >> 3) << 17);
+                    const uint64_t dq = umma_desc(s_q + s * TILE);
+                    for (int j = g; ok && j < n; j += LANES) {
+                        if (st == 0 && !(ok = wait(ms.k_full[g], (loads - 1) & 1))) break;
+                        if (mine && !(ok = wait(ms.s_free[g], (mine - 1) & 1))) break;
+                        ++mine;
+                        tc_after_sync();
+                        if (leader) {
+#pragma unroll
+                            for (int kk = 0; kk < HD / 16; ++kk) {
+                                const uint32_t off = ((kk >> 2) * ATOM + (kk & 3) * 32) >> 4;
+                                umma_ss(t_s, dk + off, dq + off, idesc, kk > 0);
+                            }
+                            umma_commit(su32(&ms.s_full[g]));
+                            if (st == stages - 1) umma_commit(su32(&ms.k_free[g]));
+                        }
+                        __syncwarp();
+                        if (st == stages - 1 && t + j + LANES < sg.t1) load(t + j + LANES);
+                    }
+                    if (!ok) break;
+                    if (leader) umma_commit(su32(&ms.q_free[s]));
+                    __syncwarp();
+                }
+                t += n;
+            }
+        }
+        if (!ok && leader) {  // leave nothing in flight: the MMAs already issued, then the last copy
+            umma_commit(su32(&ms.drain[g]));
+            mb_wait(su32(&ms.drain[g]), 0);
+            if (loads) mb_wait(su32(&ms.k_full[g]), (loads - 1) & 1);
+        }
     } else {
-        const int w = (warp - 4) >> 2, key_in = 32 * (warp & 3) + lane;  // tiles of parity w
-        const uint32_t t_s = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * w;
+        const int g = (warp - 4) >> 2, key_in = 32 * (warp & 3) + lane;
+        const uint32_t t_s = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * g;
         const float c2 = p.scale * LOG2E;
         uint32_t fill = 0, mine = 0;
         bool ok = true;
@@ -329,48 +315,31 @@ __global__ void __launch_bounds__(XT, 1)
             const int past = sg.past - key_in, end = past + p.n_nodes;  // of keys counted from key_in
             for (int t = sg.t0; ok && t < sg.t1;) {
                 const int n = min(set_of(stages), sg.t1 - t);
-                float acc[2] = {0.f, 0.f};  // several stages: of the set's tiles w and w + 2
+                float acc = 0.f;
                 for (int st = 0; ok && st < stages; ++st, ++fill) {
                     const uint32_t rs = fill % NR;
                     if (!(ok = wait(ms.r_full[rs], (fill / NR) & 1))) break;
-                    const int cols = rows - 128 * st;
-                    // Two tiles at a time: a row's constant, a broadcast read of shared memory, serves both
-                    // (one read a score would keep shared memory busier than the exponentials).
-                    for (int j = w; ok && j < n; j += 4) {
-                        const int key0 = (t + j) * KV_TILE, cnt = j + 2 < n ? 2 : 1;
-                        const uint32_t b0 = mine & 1, b1 = b0 ^ 1;
-                        float old0 = 0.f, old1 = 0.f;
-                        if (stages == 1) {
-                            if (key0 < past) old0 = mp[key0];
-                            if (cnt == 2 && key0 + 2 * KV_TILE < past) old1 = mp[key0 + 2 * KV_TILE];
-                        }
-                        ok = wait(ms.s_full[w + 2 * b0], (mine >> 1) & 1);
-                        if (ok && cnt == 2) ok = wait(ms.s_full[w + 2 * b1], ((mine + 1) >> 1) & 1);
-                        if (!ok) break;
+                    const int cols = min(128, rows - 128 * st);
+                    for (int j = g; j < n; j += LANES, ++mine) {
+                        const int key0 = (t + j) * KV_TILE;
+                        const bool tail = key0 + KV_TILE > sg.past;
+                        float old = 0.f;
+                        if (stages == 1 && key0 < past) old = mp[key0];
+                        if (!(ok = wait(ms.s_full[g], mine & 1))) break;
                         tc_after_sync();
-                        const bool tail = key0 + (2 * cnt - 1) * KV_TILE > sg.past;
-                        float s0[2] = {0.f, 0.f}, s1[2] = {0.f, 0.f};
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-                        for (int c = 0; c < 128; c += 64) {
-                            // columns past the stage's rows hold scores of zeros, or of constant -inf
-                            const bool on = c < cols, last = c + 64 >= min(cols, 128);
-                            if (!on) break;
-                            uint32_t va[2][32], vb[2][32];
-                            tmem_ld32(t_s + 256 * b0 + c, va[0]);
-                            tmem_ld32(t_s + 256 * b0 + c + 32, va[1]);
-                            tmem_ld32(t_s + 256 * b1 + c, vb[0]);
-                            tmem_ld32(t_s + 256 * b1 + c + 32, vb[1]);
+                        for (int c = 0; c < cols; c += 64) {
+                            // columns past the rows: scores of zero rows, constant -inf
+                            uint32_t v[2][32];
+                            tmem_ld32(t_s + c, v[0]);
+                            tmem_ld32(t_s + c + 32, v[1]);
                             tmem_wait_ld();
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                tmem_pin32(va[h]);
-                                tmem_pin32(vb[h]);
-                            }
-                            if (last) {  // read: the MMAs may use the buffers again
+                            tmem_pin32(v[0]);
+                            tmem_pin32(v[1]);
+                            if (c + 64 >= cols) {  // read: the MMAs may use the buffer again
                                 tc_before_sync();
-                                arrive_warp(ms.s_free[w + 2 * b0]);
-                                if (cnt == 2) arrive_warp(ms.s_free[w + 2 * b1]);
-                                if (w == 0 && mine == 0) arrive_warp(ms.stagger);
+                                arrive_warp(ms.s_free[g]);
                             }
                             if (tail) {
                                 // A tree row counts where the query's node sees it: the warp's 32 keys that query
@@ -379,64 +348,36 @@ __global__ void __launch_bounds__(XT, 1)
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) {
                                     const int col = c + 32 * h + lane, u0 = key0 + key_in - lane - sg.past;
-                                    const uint32_t* words = ms.seen[rs][col];
-                                    const bool counts = ms.bias[rs][col] != -INFINITY;
-                                    const uint32_t sa = transpose32(counts ? keys_seen(words, u0) : 0u);
-                                    const uint32_t sb = transpose32(counts ? keys_seen(words, u0 + 2 * KV_TILE) : 0u);
+                                    const uint32_t sees =
+                                        transpose32(ms.bias[rs][col] != -INFINITY ? keys_seen(ms.seen[rs][col], u0) : 0u);
 #pragma unroll
-                                    for (int x = 0; x < 32; ++x) {
-                                        if (!(sa & (1u << x))) va[h][x] = 0xFF800000u;
-                                        if (!(sb & (1u << x))) vb[h][x] = 0xFF800000u;
-                                    }
+                                    for (int x = 0; x < 32; ++x)
+                                        if (!(sees & (1u << x))) v[h][x] = 0xFF800000u;
                                 }
                             }
                             const float4* f = reinterpret_cast<const float4*>(ms.bias[rs] + c);
-                            if (cnt == 2) {
 #pragma unroll
-                                for (int x = 0; x < 16; ++x) {
-                                    const float4 q = f[x];
-                                    const uint32_t *a = va[x >> 3] + 4 * (x & 7), *b = vb[x >> 3] + 4 * (x & 7);
-                                    s0[0] += ex2(fmaf(__uint_as_float(a[0]), c2, q.x));
-                                    s1[0] += ex2(fmaf(__uint_as_float(b[0]), c2, q.x));
-                                    s0[1] += ex2(fmaf(__uint_as_float(a[1]), c2, q.y));
-                                    s1[1] += ex2(fmaf(__uint_as_float(b[1]), c2, q.y));
-                                    s0[0] += ex2(fmaf(__uint_as_float(a[2]), c2, q.z));
-                                    s1[0] += ex2(fmaf(__uint_as_float(b[2]), c2, q.z));
-                                    s0[1] += ex2(fmaf(__uint_as_float(a[3]), c2, q.w));
-                                    s1[1] += ex2(fmaf(__uint_as_float(b[3]), c2, q.w));
-                                }
-                            } else {
-#pragma unroll
-                                for (int x = 0; x < 16; ++x) {
-                                    const float4 q = f[x];
-                                    const uint32_t* a = va[x >> 3] + 4 * (x & 7);
-                                    s0[0] += ex2(fmaf(__uint_as_float(a[0]), c2, q.x));
-                                    s0[1] += ex2(fmaf(__uint_as_float(a[1]), c2, q.y));
-                                    s0[0] += ex2(fmaf(__uint_as_float(a[2]), c2, q.z));
-                                    s0[1] += ex2(fmaf(__uint_as_float(a[3]), c2, q.w));
-                                }
+                            for (int x = 0; x < 16; ++x) {
+                                const float4 q = f[x];
+                                const uint32_t* a = v[x >> 3] + 4 * (x & 7);
+                                sum[0] += ex2(fmaf(__uint_as_float(a[0]), c2, q.x));
+                                sum[1] += ex2(fmaf(__uint_as_float(a[1]), c2, q.y));
+                                sum[2] += ex2(fmaf(__uint_as_float(a[2]), c2, q.z));
+                                sum[3] += ex2(fmaf(__uint_as_float(a[3]), c2, q.w));
                             }
                         }
-                        mine += cnt;
-                        const float all0 = s0[0] + s0[1], all1 = s1[0] + s1[1];
-                        if (stages == 1) {
-                            if (key0 < end) mp[key0] = old0 + all0;
-                            if (cnt == 2 && key0 + 2 * KV_TILE < end) mp[key0 + 2 * KV_TILE] = old1 + all1;
-                        } else {
-                            acc[0] += all0;
-                            acc[1] += all1;
-                        }
+                        const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        if (stages > 1) acc += all;
+                        else if (key0 < end) mp[key0] = old + all;
                     }
                     if (ok) arrive_warp(ms.r_free[rs]);
                 }
                 if (!ok) break;
-                if (stages != 1) {  // none or several
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int j = w + 2 * x, key0 = (t + j) * KV_TILE;
-                        if (j < n && key0 < end) mp[key0] = (key0 < past ? mp[key0] : 0.f) + acc[x];
+                if (stages != 1)  // none or several
+                    for (int j = g; j < n; j += LANES) {
+                        const int key0 = (t + j) * KV_TILE;
+                        if (key0 < end) mp[key0] = (key0 < past ? mp[key0] : 0.f) + acc;
                     }
-                }
                 t += n;
             }
         }
