@@ -42,7 +42,7 @@ struct MmaSmem {
     static constexpr int OFF_MISC = OFF_KV + ST * TILE;
     struct Misc {
         uint64_t full[ST], empty[ST], vok[BAD_SETS];
-        uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2], flag_ok[2], drain[2], join, q_full[2], q_free, stagger;
+        uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2], flag_ok[2], drain[2], join, q_full[2], q_free[2], stagger;
         Share share;
         Shares all;
         JoinPlan plan;
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(XT, 1)
     if (tid == 0) {
         for (int i = 0; i < ST; ++i) {
             mb_init(su32(&ms.full[i]), 1);
-            mb_init(su32(&ms.empty[i]), (two ? 2 : 1) + 1);  // both groups' issuers, or one, and the cleaner
+            mb_init(su32(&ms.empty[i]), 3);  // both groups' issuers and the cleaner
         }
         for (int i = 0; i < BAD_SETS; ++i) mb_init(su32(&ms.vok[i]), 1);
         for (int w = 0; w < 2; ++w) {
@@ -98,7 +98,9 @@ __global__ void __launch_bounds__(XT, 1)
         mb_init(su32(&ms.q_full[0]), 1);
         mb_init(su32(&ms.q_full[1]), 1);
         mb_init(su32(&ms.stagger), 4);
-        mb_init(su32(&ms.q_free), 10);  // both issuers, and the groups' warps, which join over Q's memory
+        // both issuers, and the groups' warps, which join over Q's memory
+        mb_init(su32(&ms.q_free[0]), 10);
+        mb_init(su32(&ms.q_free[1]), 10);
         ms.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(XT, 1)
             // of one tile row take the two places in turn, ahead of time after a unit of a single key tile
             // (which needs no join over Q's memory).
             const uint32_t before = units == 0 ? 0 : !two && n_before == 1 ? units - 1 : units;
-            for (; ok && freed < before; ++freed) ok = wait_all(ms.q_free, freed & 1);
+            for (; ok && freed < before; ++freed) ok = wait_all(ms.q_free[freed & 1], (freed >> 1) & 1);
             if (!ok) break;
             n_before = n;
             if (lane == 0) {
@@ -191,10 +193,16 @@ __global__ void __launch_bounds__(XT, 1)
         const uint32_t t_s = tmem + 128 * w, t_o = tmem + 256 + 128 * w;
         uint64_t dq = 0;
         uint32_t base = 0, done = 0, units = 0, ord = 0, landed = 0;
+        int n = 0;
         bool ok = true;
-        auto full = [&](uint32_t pos) {  // the tiles up to ring position pos
-            for (; landed <= pos; ++landed)
+        // The unit's tiles up to ring position pos. A wait by parity tells a phase only from its neighbours, so
+        // the issuer sees every tile land, in order, and a tile of the other group's is not replaced before
+        // it has: it arrives at once for those that it does not use.
+        auto full = [&](uint32_t pos) {
+            for (; landed <= pos; ++landed) {
                 if (!wait_all(ms.full[landed % ST], (landed / ST) & 1)) return false;
+                if (!two && (tile_at(landed - base, n) & 1) != w && leader) mb_arrive(su32(&ms.empty[landed % ST]));
+            }
             return true;
         };
         auto qk = [&](uint32_t pos, int h) {
@@ -207,7 +215,8 @@ __global__ void __launch_bounds__(XT, 1)
             umma_commit(su32(&ms.s_full[w][h]));
         };
         while (ok && share.next(p, sg)) {
-            const int n = sg.t1 - sg.t0, first_tail = max(0, sg.past / KV_TILE - sg.t0);
+            const int first_tail = max(0, sg.past / KV_TILE - sg.t0);
+            n = sg.t1 - sg.t0;
             int i = two ? 0 : w;
             if (!(ok = wait_all(ms.q_full[units & 1], (units >> 1) & 1))) break;
             dq = umma_desc(s_q + (two ? w : units & 1) * TILE);
@@ -256,7 +265,8 @@ __global__ void __launch_bounds__(XT, 1)
                 ++done;
             }
             if (!ok) break;
-            if (leader) umma_commit(su32(&ms.q_free));
+            if (!(ok = full(base + 2 * n - 1))) break;
+            if (leader) umma_commit(su32(&ms.q_free[units & 1]));
             ++units;
             base += 2 * n;
             ord += n - min(n, first_tail);
@@ -338,7 +348,7 @@ __global__ void __launch_bounds__(XT, 1)
         const float c2 = p.scale * LOG2E, grow = GROW / c2;
         const int step = two ? 1 : 2;
         uint32_t done = 0, tails = 0, ord = 0;  // tiles of this group; its tail tiles; the CTA's tail tiles
-        uint32_t joins = 0;
+        uint32_t joins = 0, units = 0;
         bool ok = true;
         auto meet = [&]() {  // both groups
             arrive_warp(ms.join);
@@ -350,6 +360,8 @@ __global__ void __launch_bounds__(XT, 1)
             const int first_tail = max(0, sg.past / KV_TILE - sg.t0);  // of the segment
             const bool mine = two || w < n;                            // the group has a tile
             float m = -INFINITY, l = 0.f;
+            // A group without a tile here does not run ahead of the other by more than the queries do.
+            if (!(ok = wait_all(ms.q_full[units & 1], (units >> 1) & 1))) break;
             for (int i = two ? 0 : w; i < n; i += step) {
                 const bool tail = i >= first_tail;
                 uint32_t see[4];  // the tile's keys that the row sees, loaded before its scores are waited for
@@ -558,7 +570,8 @@ __global__ void __launch_bounds__(XT, 1)
             }
             tc_before_sync();
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive_warp(ms.q_free);
+            arrive_warp(ms.q_free[units & 1]);
+            ++units;
         }
     }
     tc_before_sync();

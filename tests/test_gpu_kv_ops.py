@@ -527,3 +527,54 @@ def test_one_workspace_for_calls_of_several_shapes(cuda):
         else:
             check_attention(q, k, v, n_past, out, lse, [None], 128 ** -0.5)
         want[t] = out
+
+
+# (dtype, head_dim, heads, kv heads, nodes, lengths): several units' parts in most CTAs. Up to 128 rows a unit, with
+# units of a single key tile in a row and between longer ones; and units of two row tiles.
+MANY_UNITS = [
+    (F16, 128, 32, 8, 26, [(37 * i) % 301 for i in range(60)]),
+    (F16, 128, 32, 8, 5, [(1, 90, 200, 700, 3)[i % 5] + i for i in range(80)]),
+    (BF16, 128, 16, 4, 12, [0, 1, 101, 102, 103, 116, 117, 245, 1200] * 9),
+    (F16, 64, 16, 4, 26, [(53 * i) % 500 for i in range(90)]),
+    (BF16, 128, 32, 8, 17, [8000 - 311 * i for i in range(8)]),
+    (F16, 128, 32, 8, 64, [(37 * i) % 301 for i in range(40)]),
+    (BF16, 64, 8, 2, 40, [(91 * i) % 640 for i in range(100)]),
+]
+
+
+@pytest.mark.parametrize("dtype,hd,nh,nkv,nodes,lengths", MANY_UNITS)
+def test_several_units_in_a_ctas_share(cuda, dtype, hd, nh, nkv, nodes, lengths):
+    """Parts of several units one behind the other in a CTA, whose roles run ahead of one another: the results
+    are right and bit for bit the same in every call."""
+    from jinf import kernels as K
+    g = gen(nodes)
+    S, mp = len(lengths), max(lengths)
+    kv_pair = make_cache(g, S, nkv, mp + nodes, hd, dtype)
+    q = torch.randn(S, nodes, nh, hd, generator=g, device="cuda", dtype=dtype)
+    n_past = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    mask = K.tree_mask(random_parents(nodes, nodes)).cuda()
+    out, lse = attend(q, *kv_pair, n_past, mp, mask)
+    K.kv_ops_status()
+    kv = K.KvView(*kv_pair)
+    ws = torch.zeros(K.tree_attention_workspace_bytes(kv, nh, nodes, mp), dtype=torch.uint8, device="cuda")
+    again, differ = torch.empty_like(out), torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(100):
+        again.fill_(math.nan)
+        K.tree_attention(again, q, kv, n_past, mp, ws, mask=mask)
+        differ += (again != out).sum()
+    K.kv_ops_status()
+    assert int(differ) == 0
+    mass = torch.zeros(S, nkv, kv.max_ctx, device="cuda")
+    first = None
+    for _ in range(20):
+        mass.zero_()
+        K.attention_mass(mass, q, kv, n_past, mp, lse, mask=mask)
+        first = mass.clone() if first is None else first
+        differ += (mass != first).sum()
+    K.kv_ops_status()
+    assert int(differ) == 0
+    at = [0, S // 3, S - 1]  # a few sequences in 64 bits
+    check_attention(q[at], kv_pair[0][at], kv_pair[1][at], n_past[at], out[at], lse[at], [mask] * 3, hd ** -0.5)
+    want, add = ref.mass(torch.zeros(3, nkv, kv.max_ctx, device="cuda"), q[at], kv_pair[0][at], [lengths[i] for i in at],
+                         [mask] * 3, lse[at], None, hd ** -0.5)
+    assert bool(((mass[at].double() - want).abs() <= 1e-4 * add + 2.0 ** -22 * want.abs()).all())
