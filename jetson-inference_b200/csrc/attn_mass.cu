@@ -6,7 +6,8 @@
 //
 // k_mass_rows: S^T = K Q^T as m16n8k16 fragments, a warp's 16 keys held in registers against the
 // query rows staged through shared memory 32 at a time. Rows of weight 0 are dropped first, so
-// the cost follows the accepted nodes, not the drafted ones.
+// the cost follows the accepted nodes, not the drafted ones. It serves what is short: one wave of CTAs
+// lives as long as its chain of node list, query rows, keys and stages, whatever the bandwidth.
 #include "kv_ops.cuh"
 
 #include <math.h>
@@ -14,7 +15,6 @@
 namespace jinf {
 namespace {
 
-constexpr int MASS_MMA_ROWS = 16;  // more query rows go to k_mass_mma (mass_mma.cu)
 constexpr int MW = 8;        // warps of a CTA, 16 keys each
 constexpr int MROWS = 32;    // query rows of a stage
 static_assert(MW * 16 == KV_TILE, "a CTA owns one tile of keys");
@@ -164,9 +164,21 @@ cudaError_t launch_mass(const TreeParams& p, const float* lse, const float* weig
 
 }  // namespace
 
+// k_mass_mma (mass_mma.cu) takes calls of more than 16 query rows a kv head, and long ones: more than five key
+// tiles for every two SMs, in units of four tiles or more. Measured (us, this kernel / k_mass_mma, 8 kv heads of
+// 128): 16 rows past 300 tokens 5.9 / 7.8, past 4000 (256 tiles) 7.8 / 8.6, 8 sequences past 600 (320) 8.1 / 9.5;
+// past 6000 (376) 13.0 / 9.1, past 32000 38 / 15, 8 sequences past 8000 55 / 18; short units: 128 sequences past 120
+// 24.1 / 24.2, 64 past 300 23.8 / 22.0 (4 rows: 22.1 / 21.5). With 32 rows past 300 tokens 7.1 / 7.7, past 4000
+// 8.6 / 8.6; with 48, 9.9 / 8.0 and 13.4 / 9.1.
+static bool use_mass_mma(const TreeParams& p) {
+    if (p.n_rows > 16) return true;
+    const int64_t unit = ((int64_t)p.max_past + p.n_nodes + KV_TILE - 1) / KV_TILE;
+    return unit >= 4 && 2 * unit * p.n_seqs * p.n_kv_heads > 5 * (int64_t)kv_device_sms();
+}
+
 cudaError_t attn_mass_launch(const TreeParams& p, bool bf, int head_dim, bool map_fits, const float* lse,
                              const float* weight, float* mass, cudaStream_t s) {
-    if (map_fits && p.n_rows > MASS_MMA_ROWS) return mass_mma_launch(p, bf, head_dim, lse, weight, mass, s);
+    if (map_fits && use_mass_mma(p)) return mass_mma_launch(p, bf, head_dim, lse, weight, mass, s);
     if (head_dim == 64) return bf ? launch_mass<true, 64>(p, lse, weight, mass, s) : launch_mass<false, 64>(p, lse, weight, mass, s);
     return bf ? launch_mass<true, 128>(p, lse, weight, mass, s) : launch_mass<false, 128>(p, lse, weight, mass, s);
 }

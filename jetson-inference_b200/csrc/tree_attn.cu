@@ -340,6 +340,8 @@ size_t tree_workspace_bytes(const TreePlan& plan, int head_dim) {
 TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_past, int sms, bool mma_fits) {
     TreePlan t;
     const int n_rows = group * n_nodes;
+    // Measured (us, k_tree_rows / k_tree_mma, heads of 128): 16 rows past 300 tokens 11.9 / 11.5, past 4000
+    // 14.6 / 15.0, past 32000 33.4 / 31.9, 4 rows past 4000 13.8 / 15.0; 32 rows 15.6 / 12.1, 17.9 / 15.0, 37.0 / 32.7
     t.mma = n_rows > 16 && mma_fits;
     if (t.mma) {  // whole nodes: two tiles of 128 rows hold 2 * (128 / group) of them
         const int most = 2 * (128 / group), blocks = (n_nodes + most - 1) / most;

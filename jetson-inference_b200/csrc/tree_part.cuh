@@ -9,7 +9,7 @@
 // The join runs at the end of the same launch, whose CTAs are all resident (cooperative launch, one
 // per SM): each CTA announces its parts, waits for those of its units and joins one slice of the
 // unit's values, so that the parts are read back by as many CTAs as wrote them, and from L2. A
-// kernel of its own for it took 5 to 8 us more a call.
+// kernel of its own for it took 2 us more a call past 4096 tokens, 5 us with 8 sequences past 8192.
 // Workspace: a counter per CTA, the slots.
 #pragma once
 

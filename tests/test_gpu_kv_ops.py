@@ -578,3 +578,36 @@ def test_several_units_in_a_ctas_share(cuda, dtype, hd, nh, nkv, nodes, lengths)
     want, add = ref.mass(torch.zeros(3, nkv, kv.max_ctx, device="cuda"), q[at], kv_pair[0][at], [lengths[i] for i in at],
                          [mask] * 3, lse[at], None, hd ** -0.5)
     assert bool(((mass[at].double() - want).abs() <= 1e-4 * add + 2.0 ** -22 * want.abs()).all())
+
+
+@pytest.mark.parametrize("dtype,hd,nh,nkv,nodes,lengths", [
+    (F16, 128, 8, 8, 1, [6100]), (BF16, 64, 32, 8, 4, [1800, 0, 513, 1801, 1, 1290, 127, 1799]),
+    (F16, 64, 12, 4, 5, [13001, 40]), (BF16, 128, 14, 2, 2, [24001])])
+@pytest.mark.parametrize("weighted", [True, False])
+def test_attention_mass_of_few_rows_over_many_tiles(cuda, dtype, hd, nh, nkv, nodes, lengths, weighted):
+    """Up to 16 query rows over hundreds of key tiles, some nodes without weight and a sequence without any."""
+    from jinf import kernels as K
+    g = gen(nodes)
+    S, mp = len(lengths), max(lengths)
+    k, v = make_cache(g, S, nkv, mp + nodes, hd, dtype)
+    for s, n in enumerate(lengths):
+        k[s, :, n + nodes:] = math.nan
+    q = torch.randn(S, nodes, nh, hd, generator=g, device="cuda", dtype=dtype)
+    n_past = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    mask = K.tree_mask(random_parents(nodes, nodes)).cuda()
+    _, lse = attend(q, k, v, n_past, mp, mask)
+    weight = None
+    if weighted:
+        weight = torch.rand(S, nodes, generator=g, device="cuda")
+        weight[:, 1::2] = 0.0
+        weight[S - 1] *= float(S == 1)
+    kv, before = K.KvView(k, v), torch.rand(S, nkv, mp + nodes, generator=g, device="cuda")
+    want, add = ref.mass(before, q, k, lengths, [mask] * S, lse, weight, hd ** -0.5)
+    first = None
+    for _ in range(20):
+        m = before.clone()
+        K.attention_mass(m, q, kv, n_past, mp, lse, mask=mask, node_weight=weight)
+        first = m if first is None else first
+        assert torch.equal(m, first)
+    K.kv_ops_status()
+    assert bool(((first.double() - want).abs() <= 1e-4 * add + 2.0 ** -22 * want.abs()).all())
