@@ -343,8 +343,20 @@ TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_p
     // Measured (us, k_tree_rows / k_tree_mma, heads of 128): 16 rows past 300 tokens 11.9 / 11.5, past 4000
     // 14.6 / 15.0, past 32000 33.4 / 31.9, 4 rows past 4000 13.8 / 15.0; 32 rows 15.6 / 12.1, 17.9 / 15.0, 37.0 / 32.7
     t.mma = n_rows > 16 && mma_fits;
-    if (t.mma) {  // whole nodes: two tiles of 128 rows hold 2 * (128 / group) of them
-        const int most = 2 * (128 / group), blocks = (n_nodes + most - 1) / most;
+    const int64_t unit = ((int64_t)max_past + n_nodes + KV_TILE - 1) / KV_TILE, all = (int64_t)n_seqs * n_kv_heads * unit;
+    if (t.mma) {  // whole nodes, 128 / group of them a tile of 128 rows
+        // Two row tiles a block (its groups share each key tile) read K and V least often; one tile a block (the
+        // groups take alternate key tiles) wastes no group on an odd number, shortens a CTA's chain and gives
+        // more CTAs something to do. One where that counts: an odd number; two tiles, unless units are long; all
+        // CTAs at one key tile each. Measured (us, two a block / one; 32 query heads on 8, 128 wide): 256 rows past
+        // 300 tokens 23.2 / 17.1, past 8000 25.4 / 22.2, 8 sequences past 8000 80 / 71, past 16000 31.5 / 29.9, past
+        // 24000 39.9 / 42.6, 8 past 32000 187 / 196; 512 rows past 300 22.0 / 17.5, past 4000 27.2 / 27.3, past
+        // 12000 39.8 / 45.7, 8 sequences past 2000 74 / 73; 1024 rows, 8 past 8000 211 / 250; odd numbers, three
+        // past 32000 79 / 67, 33 nodes of 64 heads past 131072 289 / 226; five past 32000 114 / 100, 8 past 2000
+        // 78 / 82; seven past 32000 143 / 131, 8 past 2000 108 / 124, past 8000 215 / 225.
+        const int tiles = (n_nodes + 128 / group - 1) / (128 / group);
+        const bool one = (tiles % 2 && tiles < 7) || (tiles == 2 && unit <= 128) || all * tiles <= sms;
+        const int blocks = one ? tiles : (tiles + 1) / 2;
         const int nodes = (n_nodes + blocks - 1) / blocks;
         t.block_rows = nodes * group;
     } else {
@@ -352,8 +364,7 @@ TreePlan tree_plan(int n_seqs, int n_kv_heads, int group, int n_nodes, int max_p
         t.block_rows = (n_rows + blocks - 1) / blocks;
     }
     t.row_blocks = (n_rows + t.block_rows - 1) / t.block_rows;
-    const int64_t tiles = ((int64_t)max_past + n_nodes + KV_TILE - 1) / KV_TILE;
-    const int64_t all = (int64_t)n_seqs * n_kv_heads * tiles, groups = sms / t.row_blocks;
+    const int64_t groups = sms / t.row_blocks;
     t.n_groups = (int)(all < groups ? all : groups);
     return t;
 }
