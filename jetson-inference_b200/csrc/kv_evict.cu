@@ -21,23 +21,25 @@ __device__ __forceinline__ uint32_t remote_u32(const uint32_t* p, int rank) {
     return v;
 }
 
-// Order of the masses as unsigned words: larger mass, larger word; NaN below everything; -0 as 0.
+// Order of the masses as unsigned words, 1 to 0xFF800000: larger mass, larger word; NaN below everything; -0 as 0.
 __device__ __forceinline__ uint32_t mass_rank(float x) {
-    if (isnan(x)) return 0u;
+    if (isnan(x)) return 1u;
     const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
 constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_BINS = 2 * SEL_THREADS;
+constexpr int SEL_BATCH = 8;  // rows of a thread read at a time
 constexpr int SEL_KEYS = 40960;  // ranks of a CTA's slice kept in shared memory; a longer slice is read again each pass
 
 // k_evict_select: the kept row numbers of one (sequence, kv head) per cluster of C CTAs, a contiguous
-// slice of the rows each. The n_pick rows of largest mass among rows n_sink .. n - n_recent - 1 by
-// radix selection, 11, 11 and 10 bits of the rank: the slices' counts are added over distributed
-// shared memory, one cluster barrier a round. Then every warp counts what it keeps of its own rows, a
-// scan over warps and CTAs gives the places, and the warps write the numbers in order.
-// Latency bounds it: the masses of 8192 rows are 32 KB. Clusters pay from about 16384 rows on (below
-// that their barriers cost more than one CTA's passes).
+// slice of the rows each. The n_keep rows of largest rank by radix selection, 11, 11 and 10 bits: the slices'
+// counts are added over distributed shared memory, one cluster barrier a round. Then every warp counts what
+// it keeps of its own rows, a scan over warps and CTAs gives the places, and the warps write the numbers
+// in order. The masses of 8192 rows are 32 KB: latency and the number of instructions a row bound it. Cycles
+// at 8192 rows: masses 2900, a round 2000 to 2300 (half of it the scan of the bins), counting 900, writing
+// 3000; with the ranks read again in every pass and the kept ends as conditions of each, 2000, 2800,
+// 3800 and 5000.
 template <int C>
 __global__ void __launch_bounds__(SEL_THREADS)
     k_evict_select(const float* __restrict__ mass, const int32_t* __restrict__ n_rows, int32_t* __restrict__ ids,
@@ -62,28 +64,57 @@ __global__ void __launch_bounds__(SEL_THREADS)
         for (int i = part * SEL_THREADS + tid; i < n; i += C * SEL_THREADS) op[i] = i;
         return;
     }
-    const int lo = n_sink, hi = n - n_recent;  // hi - lo > n_keep - n_sink - n_recent >= 0
     // rows of this CTA: whole warps' spans, so that a warp's rows are consecutive
     const int span = (n + C * SEL_THREADS - 1) / (C * SEL_THREADS) * 32;  // rows of a warp
     const int base = part * SEL_WARPS * span, limit = min(n, base + SEL_WARPS * span);
-    const bool stage = SEL_WARPS * span <= n_keys;
-    if (stage)
-        for (int i = base + tid; i < limit; i += SEL_THREADS) keys[i - base] = mass_rank(mp[i]);
-    auto rank_of = [&](int i) { return stage ? keys[i - base] : mass_rank(mp[i]); };
+    const int first = base + warp * span, steps = span / 32;
+    // The same thread reads a row's rank in every pass: from registers where it has SEL_BATCH rows at most, else
+    // from shared memory, or from the masses again. The first and the last rows rank above every mass and what
+    // lies past the slice below, so that what stays is the n_keep rows of largest rank.
+    const bool once = steps <= SEL_BATCH, stage = SEL_WARPS * span <= n_keys;
+    uint32_t r[SEL_BATCH];
+    auto ranks = [&](int s0) {  // of the masses
+        float x[SEL_BATCH];
+#pragma unroll
+        for (int j = 0; j < SEL_BATCH; ++j) {
+            const int i = first + 32 * (s0 + j) + lane;
+            x[j] = s0 + j < steps && i < limit ? mp[i] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < SEL_BATCH; ++j) {
+            const int i = first + 32 * (s0 + j) + lane;
+            r[j] = s0 + j >= steps || i >= limit ? 0u : i < n_sink || i >= n - n_recent ? 0xFFFFFFFFu : mass_rank(x[j]);
+        }
+    };
+    uint32_t* own = keys + warp * span + lane;
+    auto read = [&](int s0) {
+        if (once) return;
+        if (!stage) return ranks(s0);
+#pragma unroll
+        for (int j = 0; j < SEL_BATCH; ++j) r[j] = s0 + j < steps ? own[32 * (s0 + j)] : 0u;
+    };
+    for (int s0 = 0; s0 < steps && (once || stage); s0 += SEL_BATCH) {
+        ranks(s0);
+        if (!once)
+#pragma unroll
+            for (int j = 0; j < SEL_BATCH; ++j)
+                if (s0 + j < steps) own[32 * (s0 + j)] = r[j];
+    }
 
-    uint32_t left = n_keep - n_sink - n_recent;  // still to be picked among the ranks that match the prefix
-    const bool none = left == 0;
+    uint32_t left = n_keep;  // still to be picked among the ranks that match the prefix
     uint32_t prefix = 0, mask = 0;
-    for (int round = 0; round < 3 && !none; ++round) {
+    for (int round = 0; round < 3; ++round) {
         const int shift = round == 0 ? 21 : round == 1 ? 10 : 0;
         const uint32_t digit = round == 2 ? 1023u : 2047u;
         uint32_t* h = hist[round & 1];
         h[tid] = 0;
         h[tid + SEL_THREADS] = 0;
         __syncthreads();
-        for (int i = max(lo, base) + tid; i < min(hi, limit); i += SEL_THREADS) {
-            const uint32_t r = rank_of(i);
-            if ((r & mask) == prefix) atomicAdd(&h[(r >> shift) & digit], 1u);
+        for (int s0 = 0; s0 < steps; s0 += SEL_BATCH) {
+            read(s0);
+#pragma unroll
+            for (int j = 0; j < SEL_BATCH; ++j)
+                if (r[j] && (r[j] & mask) == prefix) atomicAdd(&h[(r[j] >> shift) & digit], 1u);
         }
         if constexpr (C > 1) cluster_barrier(); else __syncthreads();
         // bins SEL_BINS - 1 - 2 tid and the one below: how many have a larger digit, and these
@@ -115,15 +146,17 @@ __global__ void __launch_bounds__(SEL_THREADS)
         left = pick[1];
     }
     // ranks above `prefix` stay; of those equal to it the first `left`
-    auto sure = [&](int i) { return i < limit && (i < lo || i >= hi || (!none && rank_of(i) > prefix)); };
-    auto equal = [&](int i) { return i < limit && i >= lo && i < hi && !none && rank_of(i) == prefix; };
-    __syncthreads();  // the staged ranks, where no round ran
-    const int first = base + warp * span;
     int n_sure = 0, n_equal = 0;
-    for (int i = first; i < first + span; i += 32) {
-        n_sure += __popc(__ballot_sync(JINF_FULL_MASK, sure(i + lane)));
-        n_equal += __popc(__ballot_sync(JINF_FULL_MASK, equal(i + lane)));
+    for (int s0 = 0; s0 < steps; s0 += SEL_BATCH) {
+        read(s0);
+#pragma unroll
+        for (int j = 0; j < SEL_BATCH; ++j) {
+            n_sure += r[j] > prefix;
+            n_equal += r[j] == prefix;
+        }
     }
+    n_sure = (int)__reduce_add_sync(JINF_FULL_MASK, (unsigned)n_sure);
+    n_equal = (int)__reduce_add_sync(JINF_FULL_MASK, (unsigned)n_equal);
     if (lane == 0) {
         wsure[warp] = n_sure;
         wequal[warp] = n_equal;
@@ -148,15 +181,28 @@ __global__ void __launch_bounds__(SEL_THREADS)
         for (int c = 0; c < part; ++c)
             add((int)remote_u32((uint32_t*)&total[0], c), (int)remote_u32((uint32_t*)&total[1], c));
     }
-    for (int w = 0; w < warp; ++w) add(wsure[w], wequal[w]);
-    for (int i = first; i < first + span; i += 32) {
-        const bool eq = equal(i + lane);
-        const uint32_t before = (1u << lane) - 1u, be = __ballot_sync(JINF_FULL_MASK, eq);
-        const bool keep = sure(i + lane) || (eq && taken + __popc(be & before) < (int)left);
-        const uint32_t bk = __ballot_sync(JINF_FULL_MASK, keep);
-        if (keep) op[place + __popc(bk & before)] = i + lane;
-        place += __popc(bk);
-        taken += __popc(be);
+    {
+        // the CTA's warps before this one: min(max(left - taken, 0), e) adds up to the same taken all at once
+        const int s = (int)__reduce_add_sync(JINF_FULL_MASK, lane < warp ? (unsigned)wsure[lane] : 0u);
+        const int e = (int)__reduce_add_sync(JINF_FULL_MASK, lane < warp ? (unsigned)wequal[lane] : 0u);
+        add(s, e);
+    }
+    const uint32_t before = (1u << lane) - 1u;
+    for (int s0 = 0; s0 < steps; s0 += SEL_BATCH) {
+        read(s0);
+#pragma unroll
+        for (int j = 0; j < SEL_BATCH; ++j) {
+            bool keep = r[j] > prefix;
+            if (n_equal > 0) {  // few warps have such rows, and counting bits is slow
+                const bool eq = r[j] == prefix;
+                const uint32_t be = __ballot_sync(JINF_FULL_MASK, eq);
+                keep |= eq && taken + __popc(be & before) < (int)left;
+                taken += __popc(be);
+            }
+            const uint32_t bk = __ballot_sync(JINF_FULL_MASK, keep);
+            if (keep) op[place + __popc(bk & before)] = first + 32 * (s0 + j) + lane;
+            place += __popc(bk);
+        }
     }
     if constexpr (C > 1) cluster_barrier();  // no CTA leaves while another may read its counts
 }
@@ -231,18 +277,17 @@ __global__ void __launch_bounds__(MV_THREADS)
         int from[CP_BATCH];
 #pragma unroll
         for (int j = 0; j < CP_BATCH; ++j) from[j] = i0 + j * LANES < n ? __ldg(ip + i0 + j * LANES) : -1;
+        uint4 x[2][CP_BATCH];
 #pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            const uint8_t* s = (v ? src.v : src.k) + so;
-            uint8_t* d = (v ? dst.v : dst.k) + dof;
-            uint4 x[CP_BATCH];
+        for (int v = 0; v < 2; ++v)
 #pragma unroll
             for (int j = 0; j < CP_BATCH; ++j)
-                if (from[j] >= 0) x[j] = __ldcs(reinterpret_cast<const uint4*>(s + from[j] * src.row));
+                if (from[j] >= 0) x[v][j] = __ldcs(reinterpret_cast<const uint4*>((v ? src.v : src.k) + so + from[j] * src.row));
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
 #pragma unroll
             for (int j = 0; j < CP_BATCH; ++j)
-                if (from[j] >= 0) __stcs(reinterpret_cast<uint4*>(d + (i0 + j * LANES) * dst.row), x[j]);
-        }
+                if (from[j] >= 0) __stcs(reinterpret_cast<uint4*>((v ? dst.v : dst.k) + dof + (i0 + j * LANES) * dst.row), x[v][j]);
         if (mass_out && c == 0) {
 #pragma unroll
             for (int j = 0; j < CP_BATCH; ++j)
@@ -328,9 +373,10 @@ cudaError_t kv_evict_launch(const KvPlanes& src, const KvPlanes& dst, bool in_pl
                             const int32_t* n_rows, int32_t* ids, int32_t* n_out, int n_seqs, int n_kv_heads,
                             int row_bytes, int n_keep, int n_sink, int n_recent, cudaStream_t s) {
     const int units = n_seqs * n_kv_heads;
-    // One CTA per head up to 16384 rows, or where the heads fill the SMs and their ranks shared memory
-    // (256 heads of 32768 rows: see below); else clusters of 8.
-    cudaError_t e = src.max_ctx <= 16384 || (src.max_ctx <= SEL_KEYS && units >= kv_device_sms())
+    // One CTA a head where its ranks fit shared memory, else clusters of 8, whose slices do up to 327680 rows.
+    // Measured (us of the whole call, 8 heads to 2048 rows of 64 columns, one CTA / a cluster): 8192 rows 11.0 / 27.1,
+    // 16384 17.2 / 27.5, 32768 27.0 / 28.1, 64 heads of 32768 35 / 111.
+    cudaError_t e = src.max_ctx <= SEL_KEYS
                         ? launch_select<1>(units, mass, n_rows, ids, n_out, n_kv_heads, src.max_ctx, n_keep, n_sink, n_recent, s)
                         : launch_select<8>(units, mass, n_rows, ids, n_out, n_kv_heads, src.max_ctx, n_keep, n_sink, n_recent, s);
     if (e != cudaSuccess) return e;
